@@ -284,6 +284,112 @@ jamhip_status jamhip_glu_device(jamhip_ctx* ctx, int act, void* gate_dev, int ld
 jamhip_status jamhip_glu_device_vector(jamhip_ctx* ctx, int act, void* gate_dev, int ldg, const void* up_dev,
                                        int ldu, int rows, int cols, int lanes);
 
+/* ---- Around attention and sampling (device pointers, context stream, not synchronized; no counterpart in jam) ------
+ * What a decoder needs between the q|k|v projection and the output projection, and after the output head: head norm and
+ * rotation, a paged key / value cache of 16, 8 or 4 bits, attention over it, and the next token. The structs are read
+ * during the call and may be reused at once; the arrays that they point to are device memory, read when the work runs.
+ * Device data that is out of range never leads an access outside the buffers described here. */
+
+/* A paged cache: one buffer of jamhip_kv_cache_bytes bytes for the keys, one for the values, both 16-byte aligned. Plane
+ * 0 holds codes [page][kv head][token of the page][row], plane 1, right after it, the f16 scales [page][kv head][token of
+ * the page][head_dim / 32] of the types that have them. A slot is page * page_tokens + token of the page.
+ *   JAMHIP_F16   a row is head_dim f16
+ *   JAMHIP_Q8_0  a row is head_dim int8; per 32 elements d = max|x| / 127, code = round to nearest even of x * (1 / d)
+ *   JAMHIP_Q4_0  a row is 16 bytes per 32 elements, byte j = element j | element 16 + j << 4, biased by 8; d = (the element
+ *                of largest magnitude, the first of equals) / -8, code = floor(x * (1 / d) + 8.5), at most 15
+ * (f32 arithmetic, d stored as f16: ggml's blocks with the scales in a plane of their own). An element stands for
+ * scale * code rounded to f16. head_dim is a multiple of 32 (F16: of 8), n_pages * page_tokens below 2^31 (else
+ * JAMHIP_EUNSUPPORTED). */
+typedef struct {
+    int   type;
+    int   kv_heads, head_dim;
+    int   page_tokens, n_pages;
+    void* k;
+    void* v;
+} jamhip_kv_cache;
+
+/* Bytes of one buffer (keys or values) of such a cache, whatever k and v hold; -1 if the description is not valid. */
+int64_t jamhip_kv_cache_bytes(const jamhip_kv_cache* cache);
+
+/* The heads of a q|k|v row. q_weight, k_weight: f32 [head_dim] of the RMS norm x * rsqrt(mean(x^2) + eps) * weight of every
+ * head, NULL = no norm. The first rope_dim elements (even, 0 = none) turn by pos * inv_freq[p], p < rope_dim / 2: pair p is
+ * (p, p + rope_dim / 2), or (2p, 2p + 1) with neighbours = 1; cos and sin are multiplied by `scale` (YaRN's attention
+ * factor, 1 otherwise). Angles are computed in 64 bits from the int32 position and the f32 frequency. head_dim is even and at
+ * most 512 (else JAMHIP_EUNSUPPORTED). */
+typedef struct {
+    int         q_heads, kv_heads, head_dim, rope_dim;
+    int         neighbours;
+    float       eps, scale;
+    const void* q_weight;
+    const void* k_weight;
+    const void* inv_freq;   /* f32 [rope_dim / 2], NULL with rope_dim 0 */
+} jamhip_qk_spec;
+
+/* Norm and rotation of n tokens' query and key heads: q [n][ldq] (q_heads * head_dim of each row) -> q_out [n][ldqo], k -> k_out
+ * likewise, f32; pos int32 [n]. An output may be its input with the same stride. With q_heads or kv_heads 0 that
+ * pair of pointers is not looked at. */
+jamhip_status jamhip_qk_norm_rope(jamhip_ctx* ctx, const jamhip_qk_spec* spec, const void* q_dev, int ldq, void* q_out_dev,
+                                  int ldqo, const void* k_dev, int ldk, void* k_out_dev, int ldko, const void* pos_dev, int n);
+
+/* The same with keys and values going to the cache: token i's into slot slots[i] (int32), each slot at most once a call;
+ * a slot outside the cache (-1 for a padding token) is not written. Keys are computed in 64 bits up to the f32 value that
+ * is quantised. spec and cache name the same kv_heads and head_dim. */
+jamhip_status jamhip_qkv_norm_rope_write(jamhip_ctx* ctx, const jamhip_qk_spec* spec, const jamhip_kv_cache* cache,
+                                         const void* q_dev, int ldq, void* q_out_dev, int ldqo, const void* k_dev, int ldk,
+                                         const void* v_dev, int ldv, const void* pos_dev, const void* slots_dev, int n);
+
+/* What slots [n] (int32) of the cache stand for, as f32 rows of kv_heads * head_dim; zeros for a slot outside the cache. k_out
+ * or v_out may be NULL. */
+jamhip_status jamhip_kv_read(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const void* slots_dev, int n, void* k_out_dev,
+                             int ldk, void* v_out_dev, int ldv);
+
+/* A ragged batch. Sequence s has the query tokens [q_offsets[s], q_offsets[s + 1]) of the call's n_tokens rows; they are the last
+ * of its seq_lens[s] own tokens, whose entries are in the cache already, at the pages of row s of seq_pages [n_seqs][ld_seq_pages].
+ * Prefix group j, the sequences [prefix_seqs[j], prefix_seqs[j + 1]), has prefix_lens[j] tokens in front of the own ones, at the
+ * pages of row j of prefix_pages; a sequence outside every group has none. max_q, max_seq_len and max_prefix_len bound the
+ * device lengths (what is longer is cut; query tokens past max_q are not computed). All arrays are int32. A page outside
+ * the cache reads as zeros. */
+typedef struct {
+    int         n_tokens, n_seqs, n_prefixes;
+    int         max_q, max_seq_len, max_prefix_len;
+    const void* q_offsets;      /* [n_seqs + 1], rising */
+    const void* seq_lens;       /* [n_seqs] */
+    const void* seq_pages;
+    int         ld_seq_pages;   /* >= max_seq_len / page_tokens, rounded up */
+    const void* prefix_seqs;    /* [n_prefixes + 1], rising */
+    const void* prefix_lens;    /* [n_prefixes] */
+    const void* prefix_pages;
+    int         ld_prefix_pages;
+} jamhip_attn_batch;
+
+/* out[t] = softmax(scale * q[t] . k) . v over the keys at or before t's position, for each of q_heads heads (a multiple of the
+ * cache's kv_heads; consecutive heads share a key head); with window > 0 only the last `window` of them. sinks: f32 [q_heads]
+ * logits that count in the softmax's sum and have no value, or NULL. A row that sees no key is zeros. q [n_tokens][ldq] and out
+ * [n_tokens][ldo] are f32 and do not overlap. What a masked entry holds, NaN and Inf included, changes nothing. A shared prefix
+ * is read once for its group where that is less work (few query tokens a sequence). head_dim 64, 96, 128, 192 or 256 (else
+ * JAMHIP_EUNSUPPORTED). */
+jamhip_status jamhip_attn_shared_prefix(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const jamhip_attn_batch* batch,
+                                        const void* q_dev, int ldq, int q_heads, float scale, int window, const void* sinks_dev,
+                                        void* out_dev, int ldo);
+
+/* Per-row sampling parameters, device arrays of `rows` entries. NULL: temperature 1, no filter. */
+typedef struct {
+    const void* temperature;   /* f32; not above 0: the first of the largest logits */
+    const void* top_k;         /* int32; 0 or less: all */
+    const void* top_p;         /* f32; 1 or more: all */
+    const void* min_p;         /* f32; 0 or less: all */
+    const void* u;             /* f32 in [0, 1): the random number of the row */
+} jamhip_sampling;
+
+/* token[r] (int32) of each row of logits [rows][ld] (f32, vocab of each). With w = exp((x - max) / temperature) in 64 bits and the
+ * row sorted by value, equal ones by index: top-k keeps the first k; of those, top-p the ones before which less than p of
+ * their sum has been summed (the first in any case); of those, min-p the ones with w >= min_p (the largest in any case). The token
+ * is the first in index order whose running sum of kept w exceeds u times their sum. logprob[r] (f32, NULL = not wanted) =
+ * x - max - log(sum of exp(x - max)), over the whole row at temperature 1. NaN counts as -Inf; a row of nothing else gives
+ * token 0. */
+jamhip_status jamhip_sample(jamhip_ctx* ctx, const void* logits_dev, int64_t ld, int rows, int vocab,
+                            const jamhip_sampling* params, void* token_dev, void* logprob_dev);
+
 /* Use `stream` (a hipStream_t; NULL = the context's own) for subsequent work of this context. */
 jamhip_status jamhip_ctx_set_stream(jamhip_ctx* ctx, void* stream);
 void*         jamhip_ctx_stream(const jamhip_ctx* ctx);

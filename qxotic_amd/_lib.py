@@ -11,8 +11,38 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libjamhip.so"
 
 _lib = None
 
-# (name, restype, argtypes) for every entry point of include/jamhip.h
 _VP, _I, _I64 = C.c_void_p, C.c_int, C.c_int64
+
+
+class KvCache(C.Structure):
+    """A paged key / value cache (jamhip_kv_cache): `type` JAM.F16, Q8_0 or Q4_0, `k` and `v` device addresses."""
+
+    _fields_ = [("type", _I), ("kv_heads", _I), ("head_dim", _I), ("page_tokens", _I), ("n_pages", _I), ("k", _VP), ("v", _VP)]
+
+
+class QkSpec(C.Structure):
+    """Head norm and rotation of a q|k|v row (jamhip_qk_spec); q_weight, k_weight and inv_freq device addresses or None."""
+
+    _fields_ = [("q_heads", _I), ("kv_heads", _I), ("head_dim", _I), ("rope_dim", _I), ("neighbours", _I), ("eps", C.c_float),
+                ("scale", C.c_float), ("q_weight", _VP), ("k_weight", _VP), ("inv_freq", _VP)]
+
+
+class AttnBatch(C.Structure):
+    """A ragged batch and its shared prefixes (jamhip_attn_batch); the arrays are device addresses of int32."""
+
+    _fields_ = [("n_tokens", _I), ("n_seqs", _I), ("n_prefixes", _I), ("max_q", _I), ("max_seq_len", _I), ("max_prefix_len", _I),
+                ("q_offsets", _VP), ("seq_lens", _VP), ("seq_pages", _VP), ("ld_seq_pages", _I), ("prefix_seqs", _VP),
+                ("prefix_lens", _VP), ("prefix_pages", _VP), ("ld_prefix_pages", _I)]
+
+
+class Sampling(C.Structure):
+    """Sampling parameters per row (jamhip_sampling), device addresses; None: temperature 1, no filter."""
+
+    _fields_ = [("temperature", _VP), ("top_k", _VP), ("top_p", _VP), ("min_p", _VP), ("u", _VP)]
+
+
+_CACHE, _SPEC, _BATCH, _SAMPLING = (C.POINTER(t) for t in (KvCache, QkSpec, AttnBatch, Sampling))
+# (name, restype, argtypes) for every entry point of include/jamhip.h
 SIGNATURES = [
     ("jamhip_device_available", _I, []),
     ("jamhip_ctx_create", _VP, [_I]),
@@ -40,6 +70,12 @@ SIGNATURES = [
     ("jamhip_mm_device_ex", _I, [_VP, _VP, _I, _I, _VP, _I, _I, _VP, _I, _I, _I, _I, _I, _VP, _I]),
     ("jamhip_glu_device", _I, [_VP, _I, _VP, _I, _VP, _I, _I, _I]),
     ("jamhip_glu_device_vector", _I, [_VP, _I, _VP, _I, _VP, _I, _I, _I, _I]),
+    ("jamhip_kv_cache_bytes", _I64, [_CACHE]),
+    ("jamhip_qk_norm_rope", _I, [_VP, _SPEC, _VP, _I, _VP, _I, _VP, _I, _VP, _I, _VP, _I]),
+    ("jamhip_qkv_norm_rope_write", _I, [_VP, _SPEC, _CACHE, _VP, _I, _VP, _I, _VP, _I, _VP, _I, _VP, _VP, _I]),
+    ("jamhip_kv_read", _I, [_VP, _CACHE, _VP, _I, _VP, _I, _VP, _I]),
+    ("jamhip_attn_shared_prefix", _I, [_VP, _CACHE, _BATCH, _VP, _I, _I, C.c_float, _I, _VP, _VP, _I]),
+    ("jamhip_sample", _I, [_VP, _VP, _I64, _I, _I, _SAMPLING, _VP, _VP]),
     ("jamhip_ctx_set_stream", _I, [_VP, _VP]),
     ("jamhip_ctx_stream", _VP, [_VP]),
     ("jamhip_ctx_synchronize", _I, [_VP]),

@@ -1,7 +1,7 @@
 """Build libjamhip.so (gfx950) in-tree with hipcc: ``python -m qxotic_amd.build``.
 
 Every translation unit is compiled for gfx950 only, with packed-FP32 instructions disabled; the
-activation quantizers, the MoE routing (top-k weights) and the gated activations additionally compile with
+activation and cache quantizers, the MoE routing (top-k weights) and the gated activations additionally compile with
 -ffp-contract=off so their f32 products round exactly where jam's and jinfer's do (a product is never fused
 into a following add unless the reference writes an fma).
 """
@@ -43,6 +43,9 @@ UNITS = {   # source -> extra flags
     "mxn.hip": [],
     "moe.hip": ["-ffp-contract=off"],
     "epilogue.hip": ["-ffp-contract=off"],
+    "qkrope.hip": ["-ffp-contract=off"],
+    "attn.hip": [],
+    "sample.hip": [],
     "readfloor.hip": [],
     "jamhip.cpp": ["-x", "hip"],
     "gguf.cpp": [],

@@ -1,0 +1,124 @@
+// Attention over the paged cache: what the kernels share. Lengths, offsets and pages are device data; whatever they hold, no
+// address leaves the cache, the page tables or the token rows (lengths are cut to the call's maxima, offsets to the tokens,
+// a page outside the cache reads as zeros).
+#pragma once
+
+#include "kvcache.h"
+#include "launch.h"
+
+namespace jamhip {
+
+struct SeqInfo {
+    int t0, nq;           // its query tokens
+    int base, len;        // tokens of its prefix, and its own
+    const int* prefix;    // page rows
+    const int* own;
+};
+
+JAMHIP_DEV int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// the last i in [0, n] with a[i] <= v, or -1 (a has n + 1 entries in rising order)
+JAMHIP_DEV int last_not_above(const int* a, int n, int v) {
+    int lo = -1, hi = n + 1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= v) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+JAMHIP_DEV int prefix_of(const Attn& g, int s) {   // the sequence's prefix group or -1
+    if (g.n_prefixes <= 0) return -1;
+    const int j = last_not_above(g.prefix_seqs, g.n_prefixes, s);
+    return j >= g.n_prefixes ? -1 : j;
+}
+
+JAMHIP_DEV SeqInfo seq_info(const Attn& g, int s) {
+    SeqInfo r;
+    r.t0 = clampi(g.q_offsets[s], 0, g.n_tokens);
+    r.nq = min(clampi(g.q_offsets[s + 1], r.t0, g.n_tokens) - r.t0, g.max_q);
+    r.len = clampi(g.seq_lens[s], 0, g.seq_cap);
+    r.own = g.seq_pages + (int64_t) s * g.ld_seq_pages;
+    const int j = prefix_of(g, s);
+    r.base = j < 0 ? 0 : clampi(g.prefix_lens[j], 0, g.prefix_cap);
+    r.prefix = j < 0 ? nullptr : g.prefix_pages + (int64_t) j * g.ld_prefix_pages;
+    return r;
+}
+
+// The sequence of token t, or -1 for one that no sequence takes.
+JAMHIP_DEV int seq_of(const Attn& g, int t) {
+    const int s = last_not_above(g.q_offsets, g.n_seqs, t);
+    return s >= g.n_seqs ? -1 : s;
+}
+
+// Row (KvView::row) of key `at` of head `head` of a sequence's prefix and own tokens together, or -1 for a bad page.
+JAMHIP_DEV int64_t entry_row(const KvView& c, const SeqInfo& r, int at, int head) {
+    const bool shared = at < r.base;
+    const int i = shared ? at : at - r.base, pg = c.page.div(i), in = i - pg * c.page.d;
+    const int p = (shared ? r.prefix : r.own)[pg];
+    return p < 0 || p >= c.n_pages ? -1 : ((int64_t) p * c.kv + head) * c.page.d + in;
+}
+
+constexpr int ATTN_ROW_FLOATS = 256 + 64;   // attn_row's shared memory: the query row, then a block's weights
+
+// One output row by one wave, every masked key left out entirely: 64 keys at a time, a key a lane for the scores, 4 elements
+// a lane for the values.
+template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, float* lds) {
+    const int lane = threadIdx.x & 63, dim = g.cache.dim, kvh = g.grp.div(head);
+    const int s = seq_of(g, t);
+    if (s < 0) return;
+    const SeqInfo r = seq_info(g, s);
+    if (t - r.t0 >= r.nq) return;
+    const int pos = r.base + r.len - r.nq + (t - r.t0);
+    const int lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(r.base + r.len, pos + 1);
+    float* qs = lds;
+    float* ps = lds + 256;
+    const float* q = g.q + t * g.ldq + (int64_t) head * dim;
+    for (int d = lane; d < dim; d += 64) qs[d] = q[d] * g.scale;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float m = -__builtin_inff(), l = 0.0f;
+    float4_t acc = {0, 0, 0, 0};
+    for (int k0 = lo; k0 < hi; k0 += 64) {
+        const int at = k0 + lane;
+        float x = -__builtin_inff();
+        const int64_t row = at < hi ? entry_row(g.cache, r, at, kvh) : -1;
+        if (at < hi) {
+            x = 0.0f;
+            if (row >= 0)
+                for (int d = 0; d < dim; d += 4) {
+                    const float4_t k = kv_load4<TYPE>(g.cache.k, g.cache.scale_off, dim, row, d);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x += qs[d + i] * k[i];
+                }
+        }
+        float top = x;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float now = fmaxf(m, top), ref = now == -__builtin_inff() ? 0.0f : now;
+        const float keep = expf(m - ref), p = at < hi ? expf(x - ref) : 0.0f;
+        l = l * keep + wave_sum(p);
+        m = now;
+        ps[lane] = p;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        acc *= keep;
+        if (4 * lane < dim)
+            for (int j = 0; j < min(64, hi - k0); j++) {
+                const int64_t rv = entry_row(g.cache, r, k0 + j, kvh);
+                if (rv >= 0) acc += kv_load4<TYPE>(g.cache.v, g.cache.scale_off, dim, rv, 4 * lane) * ps[j];
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (g.sinks != nullptr) {
+        const float x = g.sinks[head], now = fmaxf(m, x), ref = now == -__builtin_inff() ? 0.0f : now, keep = expf(m - ref);
+        l = l * keep + expf(x - ref);
+        acc *= keep;
+    }
+    if (4 * lane < dim) {
+        float* o = g.out + t * g.ldo + (int64_t) head * dim + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = l == 0.0f ? 0.0f : acc[i] / l;   // a row that sees nothing is zeros
+    }
+}
+
+}  // namespace jamhip

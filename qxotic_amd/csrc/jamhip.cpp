@@ -1142,6 +1142,186 @@ jamhip_status moe_topk_impl(jamhip_ctx* ctx, void* sel, const void* wts, int row
     return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "topk launch");
 }
 
+// ------------------------------------------------------------------ around attention and sampling
+jamhip_status kv_valid(jamhip_ctx* ctx, const char* who, const jamhip_kv_cache* c, bool buffers) {
+    const std::string w(who);
+    if (!c) return fail(ctx, JAMHIP_EINVAL, w + ": null cache");
+    if (c->kv_heads <= 0 || c->head_dim <= 0 || c->page_tokens <= 0 || c->n_pages <= 0)
+        return fail(ctx, JAMHIP_EINVAL, w + ": bad cache shape");
+    if (buffers && (!c->k || !c->v)) return fail(ctx, JAMHIP_EINVAL, w + ": null cache buffer");
+    if (buffers && ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15))
+        return fail(ctx, JAMHIP_EINVAL, w + ": cache buffers must be 16-byte aligned");
+    if (c->type != F16 && c->type != Q8_0 && c->type != Q4_0)
+        return fail(ctx, JAMHIP_EUNSUPPORTED, w + ": the cache is F16, Q8_0 or Q4_0");
+    if (c->head_dim % (c->type == F16 ? 8 : 32))
+        return fail(ctx, JAMHIP_EUNSUPPORTED, w + ": head_dim must be a multiple of 32 (F16: of 8)");
+    if ((int64_t) c->kv_heads * c->head_dim > INT32_MAX / 4 || (int64_t) c->n_pages * c->page_tokens > INT32_MAX)
+        return fail(ctx, JAMHIP_EUNSUPPORTED, w + ": cache beyond 32-bit slots");
+    return JAMHIP_OK;
+}
+
+KvView kv_view(const jamhip_kv_cache* c) {
+    KvView v;
+    v.k = static_cast<uint8_t*>(c->k);
+    v.v = static_cast<uint8_t*>(c->v);
+    v.scale_off = (int64_t) c->n_pages * c->page_tokens * c->kv_heads * kv_row_bytes(c->type, c->head_dim);
+    v.kv = c->kv_heads;
+    v.dim = c->head_dim;
+    v.n_pages = c->n_pages;
+    v.page = FastDiv(c->page_tokens);
+    return v;
+}
+
+jamhip_status spec_valid(jamhip_ctx* ctx, const char* who, const jamhip_qk_spec* s, int n) {
+    const std::string w(who);
+    if (!s) return fail(ctx, JAMHIP_EINVAL, w + ": null spec");
+    if (n < 0 || s->q_heads < 0 || s->kv_heads < 0 || s->q_heads + (int64_t) s->kv_heads <= 0 || s->head_dim <= 0 || s->rope_dim < 0 ||
+        s->rope_dim > s->head_dim || s->rope_dim % 2 || (s->neighbours != 0 && s->neighbours != 1))
+        return fail(ctx, JAMHIP_EINVAL, w + ": bad shape");
+    if (s->rope_dim > 0 && !s->inv_freq) return fail(ctx, JAMHIP_EINVAL, w + ": null inv_freq");
+    if (s->head_dim % 2 || s->head_dim > 512) return fail(ctx, JAMHIP_EUNSUPPORTED, w + ": head_dim must be even and at most 512");
+    if ((int64_t) s->q_heads + 2 * (int64_t) s->kv_heads > 65535) return fail(ctx, JAMHIP_EUNSUPPORTED, w + ": too many heads");
+    return JAMHIP_OK;
+}
+
+QkRope qk_args(const jamhip_qk_spec* s, int n) {
+    QkRope g{};
+    g.qw = static_cast<const float*>(s->q_weight);
+    g.kw = static_cast<const float*>(s->k_weight);
+    g.inv_freq = static_cast<const float*>(s->inv_freq);
+    g.n = n;
+    g.q_heads = s->q_heads;
+    g.kv_heads = s->kv_heads;
+    g.dim = s->head_dim;
+    g.rot = s->rope_dim;
+    g.neighbours = s->neighbours;
+    g.eps = s->eps;
+    g.scale = s->scale;
+    return g;
+}
+
+// a row operand of `heads` heads: not looked at without heads
+bool row_bad(const void* p, int64_t ld, int64_t heads, int dim) { return heads > 0 && (!p || ld < heads * dim); }
+
+jamhip_status qk_norm_rope_impl(jamhip_ctx* ctx, const jamhip_qk_spec* s, const void* q, int ldq, void* qo, int ldqo, const void* k,
+                                int ldk, void* ko, int ldko, const void* pos, int n) {
+    if (!ctx) return JAMHIP_EINVAL;
+    jamhip_status st = spec_valid(ctx, "qk_norm_rope", s, n);
+    if (st != JAMHIP_OK) return st;
+    if (row_bad(q, ldq, s->q_heads, s->head_dim) || row_bad(qo, ldqo, s->q_heads, s->head_dim) ||
+        row_bad(k, ldk, s->kv_heads, s->head_dim) || row_bad(ko, ldko, s->kv_heads, s->head_dim))
+        return fail(ctx, JAMHIP_EINVAL, "qk_norm_rope: null operand or stride below the heads' elements");
+    if (s->rope_dim > 0 && !pos) return fail(ctx, JAMHIP_EINVAL, "qk_norm_rope: null positions");
+    if (n == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    QkRope g = qk_args(s, n);
+    if (s->q_heads > 0) g.q = (const float*) q, g.ldq = ldq, g.qo = (float*) qo, g.ldqo = ldqo;
+    if (s->kv_heads > 0) g.k = (const float*) k, g.ldk = ldk, g.ko = (float*) ko, g.ldko = ldko;
+    g.pos = (const int*) pos;
+    const hipError_t e = launch_qk_norm_rope(-1, g, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "qk_norm_rope launch");
+}
+
+jamhip_status qkv_write_impl(jamhip_ctx* ctx, const jamhip_qk_spec* s, const jamhip_kv_cache* c, const void* q, int ldq, void* qo,
+                             int ldqo, const void* k, int ldk, const void* v, int ldv, const void* pos, const void* slots, int n) {
+    if (!ctx) return JAMHIP_EINVAL;
+    jamhip_status st = spec_valid(ctx, "qkv_norm_rope_write", s, n);
+    if (st != JAMHIP_OK || (st = kv_valid(ctx, "qkv_norm_rope_write", c, true)) != JAMHIP_OK) return st;
+    if (s->kv_heads != c->kv_heads || s->head_dim != c->head_dim)
+        return fail(ctx, JAMHIP_EINVAL, "qkv_norm_rope_write: spec and cache differ in kv_heads or head_dim");
+    if (row_bad(q, ldq, s->q_heads, s->head_dim) || row_bad(qo, ldqo, s->q_heads, s->head_dim) ||
+        row_bad(k, ldk, s->kv_heads, s->head_dim) || row_bad(v, ldv, s->kv_heads, s->head_dim) || !slots)
+        return fail(ctx, JAMHIP_EINVAL, "qkv_norm_rope_write: null operand or stride below the heads' elements");
+    if (s->rope_dim > 0 && !pos) return fail(ctx, JAMHIP_EINVAL, "qkv_norm_rope_write: null positions");
+    if (n == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    QkRope g = qk_args(s, n);
+    if (s->q_heads > 0) g.q = (const float*) q, g.ldq = ldq, g.qo = (float*) qo, g.ldqo = ldqo;
+    g.k = (const float*) k, g.ldk = ldk, g.v = (const float*) v, g.ldv = ldv;
+    g.pos = (const int*) pos;
+    g.slots = (const int*) slots;
+    g.cache = kv_view(c);
+    const hipError_t e = launch_qk_norm_rope(c->type, g, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "qkv_norm_rope_write launch");
+}
+
+jamhip_status kv_read_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const void* slots, int n, void* ko, int ldk, void* vo, int ldv) {
+    if (!ctx) return JAMHIP_EINVAL;
+    const jamhip_status st = kv_valid(ctx, "kv_read", c, true);
+    if (st != JAMHIP_OK) return st;
+    const int64_t w = (int64_t) c->kv_heads * c->head_dim;
+    if (n < 0 || !slots || (!ko && !vo) || (ko && ldk < w) || (vo && ldv < w))
+        return fail(ctx, JAMHIP_EINVAL, "kv_read: null operand, negative count or stride below a token's elements");
+    if (n == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    const hipError_t e = launch_kv_read(c->type, kv_view(c), (const int*) slots, n, (float*) ko, ldk, (float*) vo, ldv, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "kv_read launch");
+}
+
+jamhip_status attn_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const jamhip_attn_batch* b, const void* q, int ldq, int heads,
+                        float scale, int window, const void* sinks, void* out, int ldo) {
+    if (!ctx) return JAMHIP_EINVAL;
+    const jamhip_status st = kv_valid(ctx, "attn", c, true);
+    if (st != JAMHIP_OK) return st;
+    if (!b || !q || !out) return fail(ctx, JAMHIP_EINVAL, "attn: null operand");
+    if (b->n_tokens < 0 || b->n_seqs < 0 || b->n_prefixes < 0 || b->max_q < 0 || b->max_seq_len < 0 || b->max_prefix_len < 0 ||
+        heads <= 0 || heads % c->kv_heads || window < 0)
+        return fail(ctx, JAMHIP_EINVAL, "attn: bad shape");
+    if (!(scale > 0.0f) || scale > 3.4e38f) return fail(ctx, JAMHIP_EINVAL, "attn: scale must be positive and finite");
+    const int64_t w = (int64_t) heads * c->head_dim;
+    if (ldq < w || ldo < w) return fail(ctx, JAMHIP_EINVAL, "attn: stride below the heads' elements");
+    auto pages = [&](int len) { return ((int64_t) len + c->page_tokens - 1) / c->page_tokens; };
+    if (b->n_seqs > 0 && (!b->q_offsets || !b->seq_lens || !b->seq_pages || b->ld_seq_pages < pages(b->max_seq_len)))
+        return fail(ctx, JAMHIP_EINVAL, "attn: null sequence array or ld_seq_pages below max_seq_len's pages");
+    if (b->n_prefixes > 0 && (!b->prefix_seqs || !b->prefix_lens || !b->prefix_pages || b->ld_prefix_pages < pages(b->max_prefix_len)))
+        return fail(ctx, JAMHIP_EINVAL, "attn: null prefix array or ld_prefix_pages below max_prefix_len's pages");
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 192 && c->head_dim != 256)
+        return fail(ctx, JAMHIP_EUNSUPPORTED, "attn: head_dim must be 64, 96, 128, 192 or 256");
+    if ((int64_t) b->max_seq_len + b->max_prefix_len > INT32_MAX - 4096 || (int64_t) b->n_tokens * heads > INT32_MAX - 4096)
+        return fail(ctx, JAMHIP_EUNSUPPORTED, "attn: lengths or rows beyond 32 bits");
+    if (b->n_tokens == 0 || b->n_seqs == 0 || b->max_q == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    Attn g{};
+    g.cache = kv_view(c);
+    g.q = (const float*) q, g.ldq = ldq, g.out = (float*) out, g.ldo = ldo;
+    g.heads = heads, g.window = window, g.scale = scale, g.sinks = (const float*) sinks;
+    g.n_tokens = b->n_tokens, g.n_seqs = b->n_seqs, g.n_prefixes = b->n_prefixes;
+    g.max_q = b->max_q < b->n_tokens ? b->max_q : b->n_tokens, g.seq_cap = b->max_seq_len, g.prefix_cap = b->max_prefix_len;
+    g.q_offsets = (const int*) b->q_offsets, g.seq_lens = (const int*) b->seq_lens, g.seq_pages = (const int*) b->seq_pages;
+    g.prefix_seqs = (const int*) b->prefix_seqs, g.prefix_lens = (const int*) b->prefix_lens;
+    g.prefix_pages = (const int*) b->prefix_pages;
+    g.ld_seq_pages = b->ld_seq_pages, g.ld_prefix_pages = b->ld_prefix_pages;
+    g.grp = FastDiv(heads / c->kv_heads);
+    const hipError_t e = launch_attn(c->type, g, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "attn launch");
+}
+
+jamhip_status sample_impl(jamhip_ctx* ctx, const void* logits, int64_t ld, int rows, int vocab, const jamhip_sampling* p,
+                          void* token, void* logprob) {
+    if (!ctx) return JAMHIP_EINVAL;
+    if (!logits || !p || !p->u || !token) return fail(ctx, JAMHIP_EINVAL, "sample: null operand");
+    if (rows < 0 || vocab <= 0 || ld < vocab) return fail(ctx, JAMHIP_EINVAL, "sample: bad shape");
+    if (rows == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    Sample g{};
+    g.logits = (const float*) logits, g.ld = ld, g.rows = rows, g.vocab = vocab;
+    g.temperature = (const float*) p->temperature, g.top_k = (const int*) p->top_k, g.top_p = (const float*) p->top_p;
+    g.min_p = (const float*) p->min_p, g.u = (const float*) p->u;
+    g.token = (int*) token, g.logprob = (float*) logprob;
+    const hipError_t e = launch_sample(g, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "sample launch");
+}
+
 jamhip_status ctx_set_stream_impl(jamhip_ctx* ctx, void* stream) {
     if (!ctx) return JAMHIP_EINVAL;
     Busy guard(ctx);   // the stream is read by every call in flight on this context
@@ -1433,6 +1613,45 @@ jamhip_status jamhip_moe_select_topk(jamhip_ctx* ctx, void* selection_dev, const
         return moe_topk_impl(x, selection_dev, weights_dev, rows, n_experts, ld, topk, mode, weights_scale,
                              expert_scale_dev, route_expert_dev, route_prob_dev, counts_dev);
     });
+}
+
+int64_t jamhip_kv_cache_bytes(const jamhip_kv_cache* c) {
+    if (kv_valid(nullptr, "kv_cache_bytes", c, false) != JAMHIP_OK) return -1;
+    return (int64_t) c->n_pages * c->page_tokens * c->kv_heads *
+           (kv_row_bytes(c->type, c->head_dim) + 2 * kv_scales(c->type, c->head_dim));
+}
+
+jamhip_status jamhip_qk_norm_rope(jamhip_ctx* ctx, const jamhip_qk_spec* spec, const void* q_dev, int ldq, void* q_out_dev,
+                                  int ldqo, const void* k_dev, int ldk, void* k_out_dev, int ldko, const void* pos_dev, int n) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) {
+        return qk_norm_rope_impl(x, spec, q_dev, ldq, q_out_dev, ldqo, k_dev, ldk, k_out_dev, ldko, pos_dev, n);
+    });
+}
+
+jamhip_status jamhip_qkv_norm_rope_write(jamhip_ctx* ctx, const jamhip_qk_spec* spec, const jamhip_kv_cache* cache,
+                                         const void* q_dev, int ldq, void* q_out_dev, int ldqo, const void* k_dev, int ldk,
+                                         const void* v_dev, int ldv, const void* pos_dev, const void* slots_dev, int n) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) {
+        return qkv_write_impl(x, spec, cache, q_dev, ldq, q_out_dev, ldqo, k_dev, ldk, v_dev, ldv, pos_dev, slots_dev, n);
+    });
+}
+
+jamhip_status jamhip_kv_read(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const void* slots_dev, int n, void* k_out_dev,
+                             int ldk, void* v_out_dev, int ldv) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) { return kv_read_impl(x, cache, slots_dev, n, k_out_dev, ldk, v_out_dev, ldv); });
+}
+
+jamhip_status jamhip_attn_shared_prefix(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const jamhip_attn_batch* batch,
+                                        const void* q_dev, int ldq, int q_heads, float scale, int window, const void* sinks_dev,
+                                        void* out_dev, int ldo) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) {
+        return attn_impl(x, cache, batch, q_dev, ldq, q_heads, scale, window, sinks_dev, out_dev, ldo);
+    });
+}
+
+jamhip_status jamhip_sample(jamhip_ctx* ctx, const void* logits_dev, int64_t ld, int rows, int vocab,
+                            const jamhip_sampling* params, void* token_dev, void* logprob_dev) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) { return sample_impl(x, logits_dev, ld, rows, vocab, params, token_dev, logprob_dev); });
 }
 
 jamhip_status jamhip_ctx_set_stream(jamhip_ctx* ctx, void* stream) {

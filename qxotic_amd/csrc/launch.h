@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "common.h"
+#include "kvcache.h"
 
 namespace jamhip {
 
@@ -248,5 +249,70 @@ hipError_t launch_moe_topk(float* sel, const float* wts, int rows, int E, int ld
 hipError_t launch_moe_combine(const float* y, int ldy, const int* route_expert, const float* route_prob,
                               const int* route_slot, int seq, int topk, int E, int dim, float* out, int ldo,
                               hipStream_t st);
+
+// Head norm, rotation and cache write (qkrope.hip). q, k, v: rows of ldq / ldk / ldv floats, n tokens; qo (and ko where the keys
+// do not go to a cache) may be the inputs themselves. inv_freq [rot / 2]; qw, kw [dim] or null; scale multiplies cos and sin.
+// type: F16, Q8_0 or Q4_0 of `cache`, or -1 (keys to ko, no v, no slots). dim <= 512.
+struct QkRope {
+    const float* q;
+    const float* k;
+    const float* v;
+    float* qo;
+    float* ko;
+    int ldq, ldk, ldv, ldqo, ldko;
+    const int* pos;
+    const int* slots;
+    const float* qw;
+    const float* kw;
+    const float* inv_freq;
+    int n, q_heads, kv_heads, dim, rot, neighbours;
+    float eps, scale;
+    KvView cache;
+    int per;   // heads of a workgroup, set by the launcher
+};
+hipError_t launch_qk_norm_rope(int type, const QkRope& g, hipStream_t st);
+
+// Entries of `slots` (outside the cache: zeros) to f32 rows [n][kv · dim]; ko or vo may be null.
+hipError_t launch_kv_read(int type, const KvView& c, const int* slots, int n, float* ko, int ldk, float* vo, int ldv,
+                          hipStream_t st);
+
+// The next token of each row of logits (sample.hip).
+struct Sample {
+    const float* logits;
+    int64_t ld;
+    int rows, vocab;
+    const float* temperature;
+    const int* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* u;
+    int* token;
+    float* logprob;
+};
+hipError_t launch_sample(const Sample& g, hipStream_t st);
+
+// Attention over the paged cache (attn.hip). Sequence s has the query tokens [q_offsets[s], q_offsets[s + 1]), the last of its
+// seq_lens[s] own tokens, whose entries its row of seq_pages lists; prefix group j, sequences [prefix_seqs[j],
+// prefix_seqs[j + 1]), has prefix_lens[j] tokens before them, listed once in row j of prefix_pages. The caps are the largest
+// lengths that the kernels look at: the caller's maxima, at most what a row of the page tables holds.
+struct Attn {
+    KvView cache;
+    const float* q;
+    float* out;
+    int64_t ldq, ldo;
+    int heads, window;
+    float scale;
+    const float* sinks;
+    int n_tokens, n_seqs, n_prefixes, max_q, seq_cap, prefix_cap;
+    const int* q_offsets;
+    const int* seq_lens;
+    const int* seq_pages;
+    const int* prefix_seqs;
+    const int* prefix_lens;
+    const int* prefix_pages;
+    int ld_seq_pages, ld_prefix_pages;
+    FastDiv grp;   // query heads per key head
+};
+hipError_t launch_attn(int type, const Attn& g, hipStream_t st);
 
 }  // namespace jamhip

@@ -26,7 +26,7 @@ from typing import Any
 import numpy as np
 
 from . import ggml
-from ._lib import lib, on_exit, register_for_teardown
+from ._lib import AttnBatch, KvCache, QkSpec, Sampling, lib, on_exit, register_for_teardown
 
 
 class JAM:
@@ -310,6 +310,38 @@ class HipJAM:
         return lib().jamhip_moe_combine(self.ctx, y_dev, ldy, route_expert_dev, route_prob_dev, route_slot_dev, seq,
                                         topk, n_experts, dim, out_dev, ldo)
 
+    # -- around attention and sampling (device pointers; jamhip.h) ----------------------------------
+    @staticmethod
+    def kv_cache_bytes(cache: KvCache) -> int:
+        """Bytes of one buffer (keys or values) of such a cache, -1 if its description is not valid (jamhip_kv_cache_bytes)."""
+        return lib().jamhip_kv_cache_bytes(cache)
+
+    def qk_norm_rope(self, spec: QkSpec, q_dev: int, ldq: int, q_out_dev: int, ldqo: int, k_dev: int, ldk: int, k_out_dev: int,
+                     ldko: int, pos_dev: int, n: int) -> int:
+        """RMS norm of every query and key head and the position rotation, one pass (jamhip_qk_norm_rope)."""
+        return lib().jamhip_qk_norm_rope(self.ctx, spec, q_dev, ldq, q_out_dev, ldqo, k_dev, ldk, k_out_dev, ldko, pos_dev, n)
+
+    def qkv_norm_rope_write(self, spec: QkSpec, cache: KvCache, q_dev: int, ldq: int, q_out_dev: int, ldqo: int, k_dev: int,
+                            ldk: int, v_dev: int, ldv: int, pos_dev: int, slots_dev: int, n: int) -> int:
+        """qk_norm_rope with the keys and values quantised into the cache's slots (jamhip_qkv_norm_rope_write)."""
+        return lib().jamhip_qkv_norm_rope_write(self.ctx, spec, cache, q_dev, ldq, q_out_dev, ldqo, k_dev, ldk, v_dev, ldv,
+                                                pos_dev, slots_dev, n)
+
+    def kv_read(self, cache: KvCache, slots_dev: int, n: int, k_out_dev: int | None, ldk: int, v_out_dev: int | None,
+                ldv: int) -> int:
+        """What slots of the cache stand for, as f32 rows (jamhip_kv_read)."""
+        return lib().jamhip_kv_read(self.ctx, cache, slots_dev, n, k_out_dev, ldk, v_out_dev, ldv)
+
+    def attn_shared_prefix(self, cache: KvCache, batch: AttnBatch, q_dev: int, ldq: int, q_heads: int, scale: float, out_dev: int,
+                           ldo: int, window: int = 0, sinks_dev: int | None = None) -> int:
+        """Attention of a ragged batch over the cache, prefixes shared by groups of sequences (jamhip_attn_shared_prefix)."""
+        return lib().jamhip_attn_shared_prefix(self.ctx, cache, batch, q_dev, ldq, q_heads, scale, window, sinks_dev, out_dev, ldo)
+
+    def sample(self, logits_dev: int, ld: int, rows: int, vocab: int, params: Sampling, token_dev: int,
+               logprob_dev: int | None = None) -> int:
+        """The next token of each row of logits from given random numbers (jamhip_sample)."""
+        return lib().jamhip_sample(self.ctx, logits_dev, ld, rows, vocab, params, token_dev, logprob_dev)
+
     def set_stream(self, stream: int | None) -> int:
         return lib().jamhip_ctx_set_stream(self.ctx, stream)
 
@@ -416,4 +448,4 @@ def addr(x) -> int:
 
 
 __all__ = ["JAM", "HipJAM", "Provider", "providers", "register", "Segment", "IllegalArgumentError",
-           "IndexOutOfBoundsError", "addr", "C"]
+           "IndexOutOfBoundsError", "addr", "C", "AttnBatch", "KvCache", "QkSpec", "Sampling"]
