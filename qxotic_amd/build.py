@@ -45,6 +45,9 @@ UNITS = {   # source -> extra flags
     "epilogue.hip": ["-ffp-contract=off"],
     "qkrope.hip": ["-ffp-contract=off"],
     "attn.hip": [],
+    "attn_f16.hip": [],
+    "attn_q8.hip": [],
+    "attn_q4.hip": [],
     "sample.hip": [],
     "readfloor.hip": [],
     "jamhip.cpp": ["-x", "hip"],

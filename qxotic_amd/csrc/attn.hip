@@ -1,32 +1,106 @@
 // Attention of a ragged batch over the paged cache, prefixes shared by groups of sequences.
 //   out = Σ_k exp(s_k - m) · v_k / (Σ_k exp(s_k - m) [+ exp(sink - m)]),  s_k = scale · q · k
-// over the keys at positions p' <= p of the query, with a window p' > p - window.
-#include "attn.h"
+// over the keys at positions p' <= p of the query, with a window p' > p - window. attn_plan.h cuts a call into workgroups,
+// attn_tile.h computes them; here the parts of a row whose keys were split are joined.
+#include "attn_tile.h"
 
 namespace jamhip {
 
 namespace {
 
-template <int TYPE> __global__ void __launch_bounds__(256) attn_rows_kernel(Attn g) {
-    __shared__ float lds[4][ATTN_ROW_FLOATS];
-    const int64_t i = (int64_t) blockIdx.x * 4 + threadIdx.x / 64;
-    if (i >= (int64_t) g.n_tokens * g.heads) return;
-    attn_row<TYPE>(g, (int) (i / g.heads), (int) (i % g.heads), lds[threadIdx.x / 64]);
+// One output row a wave: its parts (m_i, l_i, o_i) joined as Σ 2^(m_i - M) o_i / Σ 2^(m_i - M) l_i over the parts whose keys it
+// sees any of (no other part was written).
+template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, AttnPlan p) {
+    __shared__ float redo[4][ATTN_ROW_FLOATS];
+    const Attn& g = a.g;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t n = (int64_t) g.n_tokens * g.heads, i = (int64_t) blockIdx.x * 4 + wave;
+    if (i >= n) return;
+    const int t = (int) (i / g.heads), head = (int) (i - (int64_t) t * g.heads);
+    const int sq = seq_of(g, t);
+    if (sq < 0) return;
+    const SeqInfo s = seq_info(g, sq);
+    if (t - s.t0 >= s.nq) return;
+    const int pos = s.base + s.len - s.nq + (t - s.t0), lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(s.base + s.len, pos + 1);
+    constexpr int E = D > 128 ? 4 : D > 64 ? 2 : 1;   // elements a lane
+    float m = -__builtin_inff(), l = 0.0f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = 0.0f;
+    for (int k = 0; k < p.n; k++) {
+        const AttnPart& q = p.part[k];
+        const int a0 = q.mode == 2 ? max(0, lo - s.base) : lo, a1 = q.mode == 2 ? hi - s.base : q.mode == 1 ? min(hi, s.base) : hi;
+        if (a0 >= a1) continue;
+        for (int c = a0 / q.chunk; c <= (a1 - 1) / q.chunk && c < q.splits; c++) {
+            const int64_t at = (int64_t) (q.slot0 + c) * n + i;
+            const float2 ml = a.ml[at];
+            if (ml.x == -__builtin_inff()) continue;
+            const float now = fmaxf(m, ml.x), keep = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+            const float w = __builtin_amdgcn_exp2f(ml.x - now);
+            m = now;
+            l = l * keep + ml.y * w;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int d = lane * E + e;
+                o[e] = o[e] * keep + (d < D ? a.acc[at * D + d] : 0.0f) * w;
+            }
+        }
+    }
+    if (g.sinks != nullptr) {
+        const float x = g.sinks[head] * LOG2E, now = fmaxf(m, x), keep = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+        l = l * keep + (now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - now + WEIGHT_EXP));
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= keep;
+    }
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        o[e] = l == 0.0f ? 0.0f : o[e] / l;
+        bad |= !(fabsf(o[e]) < __builtin_inff());
+        const int d = lane * E + e;
+        if (d < D) g.out[(int64_t) t * g.ldo + (int64_t) head * D + d] = o[e];
+    }
+    if (__any(bad)) attn_row<TYPE>(g, t, head, redo[wave]);
+}
+
+template <int TYPE> hipError_t launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+    const uint32_t blocks = (uint32_t) (((int64_t) a.g.n_tokens * a.g.heads + 3) / 4);
+    switch (a.g.cache.dim) {
+        case 64: attn_join_kernel<TYPE, 64><<<blocks, 256, 0, st>>>(a, p); break;
+        case 96: attn_join_kernel<TYPE, 96><<<blocks, 256, 0, st>>>(a, p); break;
+        case 128: attn_join_kernel<TYPE, 128><<<blocks, 256, 0, st>>>(a, p); break;
+        case 192: attn_join_kernel<TYPE, 192><<<blocks, 256, 0, st>>>(a, p); break;
+        case 256: attn_join_kernel<TYPE, 256><<<blocks, 256, 0, st>>>(a, p); break;
+        default: return hipErrorNotSupported;
+    }
+    return hipGetLastError();
+}
+
+AttnPlan plan_of(const Attn& g) {
+    return attn_plan(g.cache.dim, g.cache.kv, g.grp.d, g.n_tokens, g.n_seqs, g.n_prefixes, g.max_q, g.seq_cap, g.prefix_cap);
 }
 
 }  // namespace
 
-hipError_t launch_attn(int type, const Attn& g, hipStream_t st) {
+size_t attn_workspace(const Attn& g) {
+    const size_t rows = (size_t) plan_of(g).slots * g.n_tokens * g.heads;
+    return rows * (g.cache.dim + 2) * sizeof(float);
+}
+
+hipError_t launch_attn(int type, const Attn& g, void* work, hipStream_t st) {
     if (g.n_tokens <= 0 || g.n_seqs <= 0) return hipSuccess;
-    const int64_t blocks = ((int64_t) g.n_tokens * g.heads + 3) / 4;
-    if (blocks > INT32_MAX) return hipErrorNotSupported;
-    switch (type) {
-        case F16: attn_rows_kernel<F16><<<(uint32_t) blocks, 256, 0, st>>>(g); break;
-        case Q8_0: attn_rows_kernel<Q8_0><<<(uint32_t) blocks, 256, 0, st>>>(g); break;
-        case Q4_0: attn_rows_kernel<Q4_0><<<(uint32_t) blocks, 256, 0, st>>>(g); break;
-        default: return hipErrorNotSupported;
+    const AttnPlan p = plan_of(g);
+    AttnArgs a;
+    a.g = g;
+    a.acc = static_cast<float*>(work);
+    a.ml = reinterpret_cast<float2*>(a.acc + (size_t) p.slots * g.n_tokens * g.heads * g.cache.dim);
+    for (int i = 0; i < p.n; i++) {
+        a.part = p.part[i];
+        const hipError_t e = type == F16 ? launch_attn_f16(a, st) : type == Q8_0 ? launch_attn_q8(a, st)
+                           : type == Q4_0 ? launch_attn_q4(a, st) : hipErrorNotSupported;
+        if (e != hipSuccess) return e;
     }
-    return hipGetLastError();
+    if (p.slots == 0) return hipSuccess;
+    return type == F16 ? launch_join<F16>(a, p, st) : type == Q8_0 ? launch_join<Q8_0>(a, p, st) : launch_join<Q4_0>(a, p, st);
 }
 
 }  // namespace jamhip

@@ -179,7 +179,7 @@ struct jamhip_ctx {
     mutable std::mutex pin_mu;
     std::vector<Pin> pins;
     int64_t pinned_bytes = 0;   // sum of pins[].bytes, under pin_mu
-    DevBuf act, gact, part, moe, route, gath; // kernel scratch (addresses may be captured in graphs)
+    DevBuf act, gact, part, moe, route, gath, attn; // kernel scratch (addresses may be captured in graphs)
     DevBuf fold;                              // the repack's fold flag (one int)
     StageBuf a_stage, c_stage, w_raw, w_stage;   // staging of host copies
     HostBuf a_host, c_host;   // jamhip_mm's pinned bounce buffers for A and C
@@ -1300,7 +1300,9 @@ jamhip_status attn_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const jamhip_
     g.prefix_pages = (const int*) b->prefix_pages;
     g.ld_seq_pages = b->ld_seq_pages, g.ld_prefix_pages = b->ld_prefix_pages;
     g.grp = FastDiv(heads / c->kv_heads);
-    const hipError_t e = launch_attn(c->type, g, ctx->stream);
+    hipError_t e = ctx->attn.ensure(attn_workspace(g));
+    if (e != hipSuccess) return hip_fail(ctx, e, "attn workspace");
+    e = launch_attn(c->type, g, ctx->attn.p, ctx->stream);
     return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "attn launch");
 }
 
@@ -1390,6 +1392,7 @@ void destroy_ctx(jamhip_ctx* ctx) {
     ctx->moe.release();
     ctx->route.release();
     ctx->gath.release();
+    ctx->attn.release();
     ctx->a_stage.release();
     ctx->c_stage.release();
     ctx->w_raw.release();

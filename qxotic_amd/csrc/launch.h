@@ -313,6 +313,7 @@ struct Attn {
     int ld_seq_pages, ld_prefix_pages;
     FastDiv grp;   // query heads per key head
 };
-hipError_t launch_attn(int type, const Attn& g, hipStream_t st);
+size_t attn_workspace(const Attn& g);   // bytes of `work`
+hipError_t launch_attn(int type, const Attn& g, void* work, hipStream_t st);
 
 }  // namespace jamhip
