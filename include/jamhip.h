@@ -383,7 +383,7 @@ typedef struct {
 
 /* token[r] (int32) of each row of logits [rows][ld] (f32, vocab of each). With w = exp((x - max) / temperature) in 64 bits and the
  * row sorted by value, equal ones by index: top-k keeps the first k; of those, top-p the ones before which less than p of
- * their sum has been summed (the first in any case); of those, min-p the ones with w >= min_p (the largest in any case). The token
+ * their sum has been summed (the first in any case); of those, min-p the ones with w >= min(min_p, 1). The token
  * is the first in index order whose running sum of kept w exceeds u times their sum. logprob[r] (f32, NULL = not wanted) =
  * x - max - log(sum of exp(x - max)), over the whole row at temperature 1. NaN counts as -Inf; a row of nothing else gives
  * token 0. */

@@ -111,8 +111,7 @@ def sample(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=0.0):
         keep = before < top_p * w.sum()
         keep[0] = True
         order, w = order[keep], w[keep]
-    keep = w >= min_p
-    keep[0] = True
+    keep = w >= min(min_p, 1.0)
     order, w = order[keep], w[keep]
     by = np.argsort(order)
     order, w = order[by], w[by]

@@ -179,7 +179,7 @@ struct jamhip_ctx {
     mutable std::mutex pin_mu;
     std::vector<Pin> pins;
     int64_t pinned_bytes = 0;   // sum of pins[].bytes, under pin_mu
-    DevBuf act, gact, part, moe, route, gath, attn; // kernel scratch (addresses may be captured in graphs)
+    DevBuf act, gact, part, moe, route, gath, attn, sample; // kernel scratch (addresses may be captured in graphs)
     DevBuf fold;                              // the repack's fold flag (one int)
     StageBuf a_stage, c_stage, w_raw, w_stage;   // staging of host copies
     HostBuf a_host, c_host;   // jamhip_mm's pinned bounce buffers for A and C
@@ -1320,7 +1320,9 @@ jamhip_status sample_impl(jamhip_ctx* ctx, const void* logits, int64_t ld, int r
     g.temperature = (const float*) p->temperature, g.top_k = (const int*) p->top_k, g.top_p = (const float*) p->top_p;
     g.min_p = (const float*) p->min_p, g.u = (const float*) p->u;
     g.token = (int*) token, g.logprob = (float*) logprob;
-    const hipError_t e = launch_sample(g, ctx->stream);
+    hipError_t e = ctx->sample.ensure(sample_workspace(g));
+    if (e != hipSuccess) return hip_fail(ctx, e, "sample workspace");
+    e = launch_sample(g, ctx->sample.p, ctx->stream);
     return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "sample launch");
 }
 
@@ -1393,6 +1395,7 @@ void destroy_ctx(jamhip_ctx* ctx) {
     ctx->route.release();
     ctx->gath.release();
     ctx->attn.release();
+    ctx->sample.release();
     ctx->a_stage.release();
     ctx->c_stage.release();
     ctx->w_raw.release();

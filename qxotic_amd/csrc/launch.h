@@ -289,7 +289,8 @@ struct Sample {
     int* token;
     float* logprob;
 };
-hipError_t launch_sample(const Sample& g, hipStream_t st);
+size_t sample_workspace(const Sample& g);   // bytes of `work`
+hipError_t launch_sample(const Sample& g, void* work, hipStream_t st);
 
 // Attention over the paged cache (attn.hip). Sequence s has the query tokens [q_offsets[s], q_offsets[s + 1]), the last of its
 // seq_lens[s] own tokens, whose entries its row of seq_pages lists; prefix group j, sequences [prefix_seqs[j],
