@@ -348,7 +348,7 @@ jamhip_status jamhip_kv_read(jamhip_ctx* ctx, const jamhip_kv_cache* cache, cons
  * Prefix group j, the sequences [prefix_seqs[j], prefix_seqs[j + 1]), has prefix_lens[j] tokens in front of the own ones, at the
  * pages of row j of prefix_pages; a sequence outside every group has none. max_q, max_seq_len and max_prefix_len bound the
  * device lengths (what is longer is cut; query tokens past max_q are not computed). All arrays are int32. A page outside
- * the cache reads as zeros. */
+ * the cache is read as page 0. */
 typedef struct {
     int         n_tokens, n_seqs, n_prefixes;
     int         max_q, max_seq_len, max_prefix_len;

@@ -1,6 +1,6 @@
 // Attention over the paged cache: what the kernels share. Lengths, offsets and pages are device data; whatever they hold, no
 // address leaves the cache, the page tables or the token rows (lengths are cut to the call's maxima, offsets to the tokens,
-// a page outside the cache reads as zeros).
+// a page outside the cache is read as page 0).
 #pragma once
 
 #include "kvcache.h"
@@ -52,12 +52,54 @@ JAMHIP_DEV int seq_of(const Attn& g, int t) {
     return s >= g.n_seqs ? -1 : s;
 }
 
-// Row (KvView::row) of key `at` of head `head` of a sequence's prefix and own tokens together, or -1 for a bad page.
+// A batch of up to 64 sequences and 64 groups in a wave's lanes: one round of loads, where a search through the arrays is a chain
+// of them (a load that misses takes 1 us, a small call's attention 4).
+struct BatchLanes {
+    int off, next, len;      // of sequence `lane`; next: the end of its query tokens
+    int cut, cut_next, plen; // of group `lane`
+};
+JAMHIP_DEV bool fits_lanes(const Attn& g) { return g.n_seqs <= 64 && g.n_prefixes <= 64; }
+JAMHIP_DEV BatchLanes batch_lanes(const Attn& g) {   // whole waves
+    const int lane = threadIdx.x & 63, s = min(lane, g.n_seqs - 1);
+    BatchLanes r;
+    const int off = g.q_offsets[s], next = g.q_offsets[s + 1], len = g.seq_lens[s];
+    r.cut = r.cut_next = r.plen = 0;
+    if (g.n_prefixes > 0) {
+        const int j = min(lane, g.n_prefixes - 1);
+        const int cut = g.prefix_seqs[j], cut_next = g.prefix_seqs[j + 1], plen = g.prefix_lens[j];
+        r.cut = clampi(cut, 0, g.n_seqs);
+        r.cut_next = lane < g.n_prefixes ? clampi(cut_next, r.cut, g.n_seqs) : r.cut;
+        r.plen = clampi(plen, 0, g.prefix_cap);
+    }
+    r.off = clampi(off, 0, g.n_tokens);
+    r.next = lane < g.n_seqs ? clampi(next, r.off, g.n_tokens) : r.off;
+    r.len = clampi(len, 0, g.seq_cap);
+    return r;
+}
+JAMHIP_DEV int lane_int(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+JAMHIP_DEV SeqInfo seq_info(const Attn& g, const BatchLanes& b, int s) {   // s the same in every lane
+    SeqInfo r;
+    r.t0 = lane_int(b.off, s);
+    r.nq = min(lane_int(b.next, s) - r.t0, g.max_q);
+    r.len = lane_int(b.len, s);
+    r.own = g.seq_pages + (int64_t) s * g.ld_seq_pages;
+    const unsigned long long in = __ballot(b.cut <= s && s < b.cut_next);
+    const int j = in ? __ffsll(in) - 1 : 0;
+    r.base = in ? lane_int(b.plen, j) : 0;
+    r.prefix = in ? g.prefix_pages + (int64_t) j * g.ld_prefix_pages : nullptr;
+    return r;
+}
+JAMHIP_DEV int seq_of(const BatchLanes& b, int t) {   // t the same in every lane
+    const unsigned long long in = __ballot(b.off <= t && t < b.next);
+    return in ? __ffsll(in) - 1 : -1;
+}
+
+// Row (KvView::row) of key `at` of head `head` of a sequence's prefix and own tokens together.
 JAMHIP_DEV int64_t entry_row(const KvView& c, const SeqInfo& r, int at, int head) {
     const bool shared = at < r.base;
     const int i = shared ? at : at - r.base, pg = c.page.div(i), in = i - pg * c.page.d;
     const int p = (shared ? r.prefix : r.own)[pg];
-    return p < 0 || p >= c.n_pages ? -1 : ((int64_t) p * c.kv + head) * c.page.d + in;
+    return ((int64_t) ((uint32_t) p < (uint32_t) c.n_pages ? p : 0) * c.kv + head) * c.page.d + in;
 }
 
 constexpr int ATTN_ROW_FLOATS = 256 + 64;   // attn_row's shared memory: the query row, then a block's weights
@@ -82,15 +124,14 @@ template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, flo
     for (int k0 = lo; k0 < hi; k0 += 64) {
         const int at = k0 + lane;
         float x = -__builtin_inff();
-        const int64_t row = at < hi ? entry_row(g.cache, r, at, kvh) : -1;
         if (at < hi) {
+            const int64_t row = entry_row(g.cache, r, at, kvh);
             x = 0.0f;
-            if (row >= 0)
-                for (int d = 0; d < dim; d += 4) {
-                    const float4_t k = kv_load4<TYPE>(g.cache.k, g.cache.scale_off, dim, row, d);
+            for (int d = 0; d < dim; d += 4) {
+                const float4_t k = kv_load4<TYPE>(g.cache.k, g.cache.scale_off, dim, row, d);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) x += qs[d + i] * k[i];
-                }
+                for (int i = 0; i < 4; i++) x += qs[d + i] * k[i];
+            }
         }
         float top = x;
 #pragma unroll
@@ -104,8 +145,8 @@ template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, flo
         acc *= keep;
         if (4 * lane < dim)
             for (int j = 0; j < min(64, hi - k0); j++) {
-                const int64_t rv = entry_row(g.cache, r, k0 + j, kvh);
-                if (rv >= 0) acc += kv_load4<TYPE>(g.cache.v, g.cache.scale_off, dim, rv, 4 * lane) * ps[j];
+                const int64_t row = entry_row(g.cache, r, k0 + j, kvh);
+                acc += kv_load4<TYPE>(g.cache.v, g.cache.scale_off, dim, row, 4 * lane) * ps[j];
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }

@@ -1,10 +1,14 @@
 // Attention of a ragged batch over the paged cache, prefixes shared by groups of sequences.
 //   out = Σ_k exp(s_k - m) · v_k / (Σ_k exp(s_k - m) [+ exp(sink - m)]),  s_k = scale · q · k
 // over the keys at positions p' <= p of the query, with a window p' > p - window. attn_plan.h cuts a call into workgroups,
-// attn_tile.h computes them; here the parts of a row whose keys were split are joined.
-#include "attn_tile.h"
+// attn_tile.h and attn_wave.h compute them; here the parts of a row whose keys were split are joined.
+#include "attn_mma.h"
 
 namespace jamhip {
+
+hipError_t launch_attn_f16(const AttnArgs& a, hipStream_t st);
+hipError_t launch_attn_q8(const AttnArgs& a, hipStream_t st);
+hipError_t launch_attn_q4(const AttnArgs& a, hipStream_t st);
 
 namespace {
 
@@ -17,31 +21,56 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
     const int64_t n = (int64_t) g.n_tokens * g.heads, i = (int64_t) blockIdx.x * 4 + wave;
     if (i >= n) return;
     const int t = (int) (i / g.heads), head = (int) (i - (int64_t) t * g.heads);
-    const int sq = seq_of(g, t);
+    const bool small = fits_lanes(g);
+    BatchLanes lanes;
+    if (small) lanes = batch_lanes(g);
+    const int sq = small ? seq_of(lanes, t) : seq_of(g, t);
     if (sq < 0) return;
-    const SeqInfo s = seq_info(g, sq);
+    const SeqInfo s = small ? seq_info(g, lanes, sq) : seq_info(g, sq);
     if (t - s.t0 >= s.nq) return;
     const int pos = s.base + s.len - s.nq + (t - s.t0), lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(s.base + s.len, pos + 1);
     constexpr int E = D > 128 ? 4 : D > 64 ? 2 : 1;   // elements a lane
     float m = -__builtin_inff(), l = 0.0f, o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = 0.0f;
+    int first[2] = {0, 0}, count[2] = {0, 0};   // workspace slots
     for (int k = 0; k < p.n; k++) {
         const AttnPart& q = p.part[k];
         const int a0 = q.mode == 2 ? max(0, lo - s.base) : lo, a1 = q.mode == 2 ? hi - s.base : q.mode == 1 ? min(hi, s.base) : hi;
         if (a0 >= a1) continue;
-        for (int c = a0 / q.chunk; c <= (a1 - 1) / q.chunk && c < q.splits; c++) {
-            const int64_t at = (int64_t) (q.slot0 + c) * n + i;
-            const float2 ml = a.ml[at];
-            if (ml.x == -__builtin_inff()) continue;
-            const float now = fmaxf(m, ml.x), keep = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
-            const float w = __builtin_amdgcn_exp2f(ml.x - now);
-            m = now;
-            l = l * keep + ml.y * w;
+        first[k] = q.slot0 + a0 / q.chunk;
+        count[k] = min((a1 - 1) / q.chunk, q.splits - 1) - a0 / q.chunk + 1;
+    }
+    const int all = count[0] + count[1];
+    for (int k0 = 0; k0 < all; k0 += 64) {   // a part a lane for the weights, then all lanes for each part's elements
+        const int k = k0 + lane, slot = k < count[0] ? first[0] + k : first[1] + k - count[0];
+        const float2 ml = k < all ? a.ml[slot * n + i] : make_float2(-__builtin_inff(), 0.0f);
+        float now = ml.x;
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int d = lane * E + e;
-                o[e] = o[e] * keep + (d < D ? a.acc[at * D + d] : 0.0f) * w;
+        for (int x = 1; x < 64; x <<= 1) now = fmaxf(now, __shfl_xor(now, x));
+        now = fmaxf(now, m);
+        const float keep = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+        const float w = ml.x == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - now);
+        m = now;
+        l = l * keep + wave_sum(ml.y * w);
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= keep;
+        const int here = min(64, all - k0);
+        for (int j0 = 0; j0 < here; j0 += 8) {   // eight loads in flight
+            float v[8][E];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int q = k0 + min(j0 + j, here - 1);
+                const float* src = a.acc + ((q < count[0] ? first[0] + q : first[1] + q - count[0]) * n + i) * D;
+#pragma unroll
+                for (int e = 0; e < E; e++) v[j][e] = D % (64 * E) == 0 || lane * E + e < D ? src[lane * E + e] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = j0 + j < here ? lane_f(w, min(j0 + j, here - 1)) : 0.0f;
+                if (x != 0.0f)   // what a part without a visible key holds is not looked at
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] += v[j][e] * x;
             }
         }
     }

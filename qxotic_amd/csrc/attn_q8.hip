@@ -1,8 +1,8 @@
-// The attention kernel over a Q8_0 cache.
-#include "attn_tile.h"
+// The attention kernels over a Q8_0 cache.
+#include "attn_launch.h"
 
 namespace jamhip {
 
-hipError_t launch_attn_q8(const AttnArgs& a, hipStream_t st) { return launch_attn_tile<Q8_0>(a, st); }
+hipError_t launch_attn_q8(const AttnArgs& a, hipStream_t st) { return launch_attn_part<Q8_0>(a, st); }
 
 }  // namespace jamhip
