@@ -97,14 +97,15 @@ template <int NC, int STEPS, typename AT> JAMHIP_DEV float load_query(const floa
         for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[st][i]));
     }
     top = column_max<NC>(top);
-    const int e = top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0;
+    const int e = max(top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0, -126);
+    const float unit = ldexpf(1.0f, -e);
 #pragma unroll
     for (int st = 0; st < STEPS; st++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float y = ldexpf(x[st][i], -e);
-            qh[st][i] = (_Float16) y;
-            ql[st][i] = (_Float16) (y - (float) qh[st][i]);
+        for (int i = 0; i < 8; i += 2) {
+            const float y = x[st][i] * unit, z = x[st][i + 1] * unit;
+            const half2_t h = pack_rtz(y, z), r = pack_rtz(y - (float) h[0], z - (float) h[1]);
+            qh[st][i] = h[0], qh[st][i + 1] = h[1], ql[st][i] = r[0], ql[st][i + 1] = r[1];
         }
     return ldexpf(scale * LOG2E, e);
 }
@@ -260,7 +261,7 @@ template <int NC, int ST, typename ACC> JAMHIP_DEV void weight_halves(const ACC 
     for (int e = 0; e < 8; e += 2) {
         const float x = NC == 32 ? sc[u / 2][8 * (u % 2) + e] : sc[2 * u + e / 4][e % 4];
         const float y = NC == 32 ? sc[u / 2][8 * (u % 2) + e + 1] : sc[2 * u + e / 4][e % 4 + 1];
-        const half2_t h = pack_rtz(x, y), r = pack_rtz(x - (float) h[0], y - (float) h[1]);
+        const half2_t h = pack_rtz(x, y), r = pack_rtz(fmaf((float) h[0], -1.0f, x), fmaf((float) h[1], -1.0f, y));   // exact; one instruction each
         ph[e] = h[0], ph[e + 1] = h[1], pl[e] = r[0], pl[e + 1] = r[1];
     }
 }
@@ -271,19 +272,36 @@ template <int NC, int DT, int STRIDE, typename M, typename ACC>
 JAMHIP_DEV void add_values(ACC (&o)[DT], const uint8_t* lv, int kb, int u, half8_t ph, half8_t pl) {
     const int lane = threadIdx.x & 63, part = lane / NC, in = lane % 16, sub = NC == 32 ? (lane / 16) % 2 : 0;
     const int key = kb + u * M::DEPTH + 4 * part + in / 4;
+    constexpr int PAIR = NC == 32 ? 2 : 1;   // two products between hi and lo of one sum, where there are registers for them
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) {
-        const int e0 = dt * NC + sub * 16 + 4 * (in % 4);
-        auto at = [&](int k) {
-            const uint8_t* p = lv + lds_at<STRIDE>(k, e0 / 8) + e0 % 8 * 2;
-            const short4_t v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4_t*) (uintptr_t) (__attribute__((address_space(3))) const uint8_t*) p);
-            return __builtin_bit_cast(half4_t, v);
-        };
-        const half8_t v = join_half(at(key), at(key + M::DEPTH / 2));
-        o[dt] = M::mma(v, ph, o[dt]);
-        o[dt] = M::mma(v, pl, o[dt]);
+    for (int d0 = 0; d0 < DT; d0 += PAIR) {
+        half8_t v[PAIR];
+#pragma unroll
+        for (int i = 0; i < PAIR && d0 + i < DT; i++) {
+            const int e0 = (d0 + i) * NC + sub * 16 + 4 * (in % 4);
+            auto at = [&](int k) {
+                const uint8_t* p = lv + lds_at<STRIDE>(k, e0 / 8) + e0 % 8 * 2;
+                const short4_t w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) short4_t*) (uintptr_t) (__attribute__((address_space(3))) const uint8_t*) p);
+                return __builtin_bit_cast(half4_t, w);
+            };
+            v[i] = join_half(at(key), at(key + M::DEPTH / 2));
+        }
+#pragma unroll
+        for (int i = 0; i < PAIR && d0 + i < DT; i++) o[d0 + i] = M::mma(v[i], ph, o[d0 + i]);
+#pragma unroll
+        for (int i = 0; i < PAIR && d0 + i < DT; i++) o[d0 + i] = M::mma(v[i], pl, o[d0 + i]);
     }
+}
+
+// ---- where a key's codes and scales are: byte offsets into the cache's buffers, made once for a key and read by every lane that
+// loads a piece of it
+struct KeyAt {
+    int64_t code, scale;
+};
+template <int TYPE, int D> JAMHIP_DEV KeyAt key_at(const KvView& c, const SeqInfo& s, int at, int head) {
+    const int64_t row = entry_row(c, s, at, head);
+    return {row * kv_row_bytes(TYPE, D), c.scale_off + row * (D / 32) * 2};
 }
 
 // ---- 16 bytes of codes of a row into shared memory as f16

@@ -24,7 +24,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
     using acc_t = typename M::acc_t;
     constexpr int NC = T::NC, KEYS = T::KEYS;
     __shared__ __align__(16) uint8_t lds[2 * T::PLANE];
-    __shared__ int64_t rows[2][KEYS];
+    __shared__ __align__(16) KeyAt rows[2][KEYS];
     __shared__ int range[2][4];
     __shared__ float redo[4][ATTN_ROW_FLOATS];
     const Attn& g = a.g;
@@ -33,7 +33,9 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
     int b = blockIdx.x;
     const int kvh = b % g.cache.kv;
     b /= g.cache.kv;
-    const int tile = b % a.part.tiles, split = b / a.part.tiles;
+    // a prefix's tiles past the last are the last workgroups; a sequence's run of keys past its end is
+    const bool rows_last = a.part.mode == 1;
+    const int tile = rows_last ? b / a.part.splits : b % a.part.tiles, split = rows_last ? b % a.part.splits : b / a.part.tiles;
     RowSet w;
     if (!attn_row_set<T::ROWS>(a, tile, &w)) return;
     const Column c = attn_column(a, w, w.r0 + wave * NC + col, kvh, split);
@@ -55,18 +57,17 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
     uint4_t kr[T::PER], vr[T::PER];
     _Float16 ks[T::PER] = {}, vs[T::PER] = {};
     // past the last key it stands for that one: no load is behind a branch, and nothing that no row sees comes in
-    auto row_of = [&](int at) { return entry_row(g.cache, w.s, min(at, hi - 1), kvh); };
-    auto fetch = [&](const int64_t* rw) {
+    auto row_of = [&](int at) { return key_at<TYPE, D>(g.cache, w.s, min(at, hi - 1), kvh); };
+    auto fetch = [&](const KeyAt* rw) {
 #pragma unroll
         for (int i = 0; i < T::PER; i++) {
             const int u = tid + 256 * i, key = u / T::UPK, ch = u % T::UPK;
-            const int64_t row = rw[T::UNITS % 256 == 0 ? key : min(key, KEYS - 1)], at = (row * T::UPK + ch) * 16;
-            kr[i] = *reinterpret_cast<const uint4_t*>(g.cache.k + at);
-            vr[i] = *reinterpret_cast<const uint4_t*>(g.cache.v + at);
+            const KeyAt row = rw[T::UNITS % 256 == 0 ? key : min(key, KEYS - 1)];
+            kr[i] = *reinterpret_cast<const uint4_t*>(g.cache.k + row.code + ch * 16);
+            vr[i] = *reinterpret_cast<const uint4_t*>(g.cache.v + row.code + ch * 16);
             if constexpr (TYPE != F16) {
-                const int64_t sc = g.cache.scale_off + (row * (D / 32) + ch * T::EPU / 32) * 2;
-                ks[i] = *reinterpret_cast<const _Float16*>(g.cache.k + sc);
-                vs[i] = *reinterpret_cast<const _Float16*>(g.cache.v + sc);
+                ks[i] = *reinterpret_cast<const _Float16*>(g.cache.k + row.scale + ch * T::EPU / 32 * 2);
+                vs[i] = *reinterpret_cast<const _Float16*>(g.cache.v + row.scale + ch * T::EPU / 32 * 2);
             }
         }
     };
@@ -88,22 +89,27 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
                 put_unit<TYPE, T::STRIDE>(lv, vr[i], vs[i], key, ch);
             }
         }
-        if (k0 + KEYS < hi) fetch(rows[buf]);
-        int64_t after = 0;
-        if (tid < KEYS && k0 + 2 * KEYS < hi) after = row_of(k0 + 2 * KEYS + tid);
+        KeyAt after = {};
+        if (k0 + KEYS < hi) {
+            fetch(rows[buf]);
+            if (tid < KEYS) after = row_of(k0 + 2 * KEYS + tid);
+        }
         __syncthreads();
         if (k0 <= c.hi && k0 + KEYS > c.lo) {
             acc_t sc[T::ST];
 #pragma unroll
-            for (int i = 0; i < T::ST; i++) {
+            for (int i = 0; i < T::ST; i++)
 #pragma unroll
                 for (int k = 0; k < M::N; k++) sc[i][k] = 0.0f;
 #pragma unroll
-                for (int st = 0; st < T::STEPS; st++) {
-                    const half8_t x = *reinterpret_cast<const half8_t*>(lk + lds_at<T::STRIDE>(i * NC + col, st * 2 + part));
-                    sc[i] = M::mma(x, qh[st], sc[i]);
-                    sc[i] = M::mma(x, ql[st], sc[i]);
-                }
+            for (int st = 0; st < T::STEPS; st++) {
+                half8_t x[T::ST];
+#pragma unroll
+                for (int i = 0; i < T::ST; i++) x[i] = *reinterpret_cast<const half8_t*>(lk + lds_at<T::STRIDE>(i * NC + col, st * 2 + part));
+#pragma unroll
+                for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], qh[st], sc[i]);
+#pragma unroll
+                for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], ql[st], sc[i]);
             }
             attn_weights<M, T::ST, T::DT, NC>(sc, o, m, l, f, c, k0, part);
 #pragma unroll

@@ -40,24 +40,24 @@ template <int TYPE, int D, int NC> struct KeyLane {
         const int s = at + PARTS * MID * NM;
         return s + 4 * part + (j >= 4 ? 16 + j - 4 : j);   // Q4_0 alone
     }
-    JAMHIP_DEV void load(const uint8_t* buf, int64_t scale_off, int64_t row, int part) {
-        const uint8_t* r = buf + row * kv_row_bytes(TYPE, D);
-        const _Float16* s = reinterpret_cast<const _Float16*>(buf + scale_off) + row * (D / 32);
+    JAMHIP_DEV void load(const uint8_t* buf, const KeyAt& row, int part) {
         // bytes per element times 2: F16 4, Q8_0 2, Q4_0 1
         constexpr int B2 = TYPE == F16 ? 4 : TYPE == Q8_0 ? 2 : 1;
         constexpr int at = PARTS * BIG * NB, at2 = at + PARTS * MID * NM;
+        const uint8_t* r = buf + row.code;
+        const uint8_t* s = buf + row.scale;
 #pragma unroll
         for (int i = 0; i < NB; i++) {
-            big[i] = *reinterpret_cast<const uint4_t*>(r + (PARTS * BIG * i + BIG * part) * B2 / 2);
-            if constexpr (TYPE != F16) sb[i] = s[(PARTS * BIG * i + BIG * part) / 32];
+            big[i] = *reinterpret_cast<const uint4_t*>(r + 16 * part + PARTS * 16 * i);
+            if constexpr (TYPE != F16) sb[i] = *reinterpret_cast<const _Float16*>(s + BIG * part / 32 * 2 + PARTS * BIG * i / 32 * 2);
         }
         if constexpr (NM > 0) {
-            mid = *reinterpret_cast<const uint2_t*>(r + (at + MID * part) * B2 / 2);
-            sm = s[(at + MID * part) / 32];
+            mid = *reinterpret_cast<const uint2_t*>(r + 8 * part + at * B2 / 2);
+            sm = *reinterpret_cast<const _Float16*>(s + MID * part / 32 * 2 + at / 32 * 2);
         }
         if constexpr (NS > 0) {
-            sml = *reinterpret_cast<const uint32_t*>(r + at2 / 2 + 4 * part);
-            ss = s[(at2 + 8 * part) / 32];
+            sml = *reinterpret_cast<const uint32_t*>(r + 4 * part + at2 / 2);
+            ss = *reinterpret_cast<const _Float16*>(s + at2 / 32 * 2);
         }
     }
     template <int ST> JAMHIP_DEV half8_t step() const {
@@ -115,7 +115,7 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
     using M = typename T::M;
     using acc_t = typename M::acc_t;
     __shared__ __align__(16) uint8_t lds[T::LDS];
-    __shared__ int64_t rows[4][2][T::KEYS];
+    __shared__ __align__(16) KeyAt rows[4][2][T::KEYS];
     __shared__ float redo[4][ATTN_ROW_FLOATS];
     const Attn& g = a.g;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -123,11 +123,17 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
     int b = blockIdx.x;
     const int kvh = b % g.cache.kv;
     b /= g.cache.kv;
-    const int tile = b % a.part.tiles, split = b / a.part.tiles;
+    // a prefix's tiles past the last are the last workgroups; a sequence's run of keys past its end is
+    const bool rows_last = a.part.mode == 1;
+    const int tile = rows_last ? b / a.part.splits : b % a.part.tiles, split = rows_last ? b % a.part.splits : b / a.part.tiles;
     RowSet w;
     if (!attn_row_set<T::ROWS>(a, tile, &w)) return;
     const Column c = attn_column(a, w, w.r0 + col, kvh, split);
     const int lo = c.lo, hi = c.hi + 1;   // the same in every wave
+
+    half8_t qh[T::STEPS], ql[T::STEPS];
+    const float f = load_query<NC>(g.q + (int64_t) c.tok * g.ldq + (int64_t) c.head * D, g.scale, qh, ql,
+                                   [&](int st, int j) { return T::K::element(st, part, j); });
 
     acc_t o[T::DT];
 #pragma unroll
@@ -136,26 +142,25 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
         for (int k = 0; k < M::N; k++) o[i][k] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
 
-    int64_t (*const rw)[T::KEYS] = rows[wave];
+    KeyAt (*const rw)[T::KEYS] = rows[wave];
     uint8_t* const lv = lds + wave * T::PLANE;
     typename T::K kf[T::ST];
     uint4_t vr[T::PER];
     _Float16 vs[T::PER] = {};
     // past the last key it stands for that one: no load is behind a branch, and nothing that no row sees comes in
-    auto row_of = [&](int at) { return entry_row(g.cache, w.s, min(at, hi - 1), kvh); };
+    auto row_of = [&](int at) { return key_at<TYPE, D>(g.cache, w.s, min(at, hi - 1), kvh); };
     auto sync = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
-    auto fetch_k = [&](const int64_t* r) {
+    auto fetch_k = [&](const KeyAt* r) {
 #pragma unroll
-        for (int i = 0; i < T::ST; i++) kf[i].load(g.cache.k, g.cache.scale_off, r[i * NC + col], part);
+        for (int i = 0; i < T::ST; i++) kf[i].load(g.cache.k, r[i * NC + col], part);
     };
-    auto fetch_v = [&](const int64_t* r) {
+    auto fetch_v = [&](const KeyAt* r) {
 #pragma unroll
         for (int i = 0; i < T::PER; i++) {
             const int u = lane + 64 * i, key = u / T::UPK, ch = u % T::UPK;
-            const int64_t row = r[T::UNITS % 64 == 0 ? key : min(key, T::KEYS - 1)];
-            vr[i] = *reinterpret_cast<const uint4_t*>(g.cache.v + (row * T::UPK + ch) * 16);
-            if constexpr (TYPE != F16)
-                vs[i] = *reinterpret_cast<const _Float16*>(g.cache.v + g.cache.scale_off + (row * (D / 32) + ch * T::EPU / 32) * 2);
+            const KeyAt row = r[T::UNITS % 64 == 0 ? key : min(key, T::KEYS - 1)];
+            vr[i] = *reinterpret_cast<const uint4_t*>(g.cache.v + row.code + ch * 16);
+            if constexpr (TYPE != F16) vs[i] = *reinterpret_cast<const _Float16*>(g.cache.v + row.scale + ch * T::EPU / 32 * 2);
         }
     };
     const int first = lo < hi ? lo + T::KEYS * wave : hi, step = 4 * T::KEYS;
@@ -165,9 +170,6 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
         fetch_k(rw[0]);
         fetch_v(rw[0]);
     }
-    half8_t qh[T::STEPS], ql[T::STEPS];
-    const float f = load_query<NC>(g.q + (int64_t) c.tok * g.ldq + (int64_t) c.head * D, g.scale, qh, ql,
-                                   [&](int st, int j) { return T::K::element(st, part, j); });
     int buf = 1;
     for (int k0 = first; k0 < hi; k0 += step, buf ^= 1) {
 #pragma unroll
@@ -183,14 +185,15 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
 #pragma unroll
             for (int k = 0; k < M::N; k++) sc[i][k] = 0.0f;
         unroll<0, T::STEPS>([&](auto st) {
+            half8_t x[T::ST];
 #pragma unroll
-            for (int i = 0; i < T::ST; i++) {
-                const half8_t x = kf[i].template step<decltype(st)::value>();
-                sc[i] = M::mma(x, qh[decltype(st)::value], sc[i]);
-                sc[i] = M::mma(x, ql[decltype(st)::value], sc[i]);
-            }
+            for (int i = 0; i < T::ST; i++) x[i] = kf[i].template step<decltype(st)::value>();
+#pragma unroll
+            for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], qh[decltype(st)::value], sc[i]);
+#pragma unroll
+            for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], ql[decltype(st)::value], sc[i]);
         });
-        int64_t after = 0;
+        KeyAt after = {};
         if (more) {
             fetch_k(rw[buf]);
             if (lane < T::KEYS && k0 + 2 * step < hi) after = row_of(k0 + 2 * step + lane);
