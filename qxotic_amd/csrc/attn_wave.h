@@ -108,9 +108,9 @@ template <int TYPE, int D, int NC> struct Wave {
 };
 
 // waves a SIMD that the registers are to leave room for
-constexpr int wave_occupancy(int type, int dim, int nc) { return dim >= 192 ? 1 : nc == 16 && (type != F16 || dim == 64) ? 3 : 2; }
+constexpr int wave_occupancy(int dim, int nc) { return dim >= 192 ? 1 : nc == 16 && dim == 64 ? 3 : 2; }
 
-template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_occupancy(TYPE, D, NC))) attn_wave_kernel(AttnArgs a) {
+template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_occupancy(D, NC))) attn_wave_kernel(AttnArgs a) {
     using T = Wave<TYPE, D, NC>;
     using M = typename T::M;
     using acc_t = typename M::acc_t;

@@ -201,6 +201,12 @@ template <typename T, int LPH, bool VEC> struct Head {
     }
 };
 
+// A head's lanes are of one wave, whose shared memory operations are done in order.
+JAMHIP_DEV void sync_wave() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // One workgroup takes heads [y · per, (y + 1) · per) of one token's q | k (| v): every 256 / LPH of them at once. TYPE -1: keys
 // go out as f32. The angles of the token are computed once per workgroup, one pair a thread.
 template <int TYPE, int LPH, bool VEC> __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(QkRope g) {
@@ -247,7 +253,7 @@ template <int TYPE, int LPH, bool VEC> __global__ void __launch_bounds__(QK_THRE
                 x.rotate(turn);
                 x.store(mine);
             }
-            __syncthreads();
+            sync_wave();
             if (h < h1 && !is_q && keep && 8 * j < g.dim) {   // whole quads: dim is a multiple of 32, or the type has no blocks
                 const int i = (h - g.q_heads) - (is_k ? 0 : g.kv_heads);
                 float v[8];
@@ -263,30 +269,43 @@ template <int TYPE, int LPH, bool VEC> __global__ void __launch_bounds__(QK_THRE
                 }
                 cache_store8<TYPE>(g.cache, is_k ? g.cache.k : g.cache.v, g.cache.row(slot, i), j, v);
             }
-            __syncthreads();
+            sync_wave();
         }
     }
 }
 
-// Slots read back: 4 elements a thread, keys in blockIdx.y 0, values in 1.
-template <int TYPE> __global__ void __launch_bounds__(256) kv_read_kernel(KvView c, const int* __restrict__ slots, int n, float* ko,
-                                                                          int ldk, float* vo, int ldv) {
+// Slots read back: 4 elements a thread of each of U tokens, whose loads are in flight together; keys in blockIdx.y 0, values in 1.
+// What many tokens bring back is more than the L2s hold and goes past them (16384 tokens of 8 x 128 in Q8_0 49 -> 30 us).
+template <int TYPE, int U> __global__ void __launch_bounds__(256) kv_read_kernel(KvView c, const int* __restrict__ slots, int n, float* ko,
+                                                                                 int ldk, float* vo, int ldv) {
     const bool is_v = blockIdx.y == 1 || ko == nullptr;
-    const int per = c.kv * c.dim / 4;   // 4-element pieces of a token
+    const int per = c.kv * c.dim / 4, step = (n + U - 1) / U;   // 4-element pieces of a token; the thread's tokens are step apart
     const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t) n * per) return;
-    const int64_t t = i / per;
-    const int p = (int) (i - t * per), head = p / (c.dim / 4), e = (p - head * (c.dim / 4)) * 4;
-    const int64_t slot = slots[t];
-    float4_t x = {0, 0, 0, 0};
-    if (slot >= 0 && slot < c.slots()) x = kv_load4<TYPE>(is_v ? c.v : c.k, c.scale_off, c.dim, c.row(slot, head), e);
-    float* o = is_v ? vo + t * ldv : ko + t * ldk;
-    o += head * c.dim + e;
-    if ((reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-        *reinterpret_cast<float4_t*>(o) = x;
-    } else {
+    const int t0 = (int) (i / per), p = (int) (i - (int64_t) t0 * per), head = p / (c.dim / 4), e = (p - head * (c.dim / 4)) * 4;
+    if (t0 >= step) return;
+    const uint8_t* buf = is_v ? c.v : c.k;
+    int64_t slot[U];
+    float4_t x[U];
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[k] = x[k];
+    for (int u = 0; u < U; u++) slot[u] = slots[min(t0 + u * step, n - 1)];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const bool in = slot[u] >= 0 && slot[u] < c.slots();
+        x[u] = kv_load4<TYPE>(buf, c.scale_off, c.dim, c.row(in ? slot[u] : 0, head), e);
+        if (!in) x[u] = float4_t{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int t = t0 + u * step;
+        if (t >= n) continue;
+        float* o = (is_v ? vo + (int64_t) t * ldv : ko + (int64_t) t * ldk) + head * c.dim + e;
+        if ((reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+            if constexpr (U > 1) __builtin_nontemporal_store(x[u], reinterpret_cast<float4_t*>(o));
+            else *reinterpret_cast<float4_t*>(o) = x[u];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] = x[u][k];
+        }
     }
 }
 
@@ -327,13 +346,20 @@ hipError_t launch_qk_norm_rope(int type, const QkRope& g, hipStream_t st) {
 hipError_t launch_kv_read(int type, const KvView& c, const int* slots, int n, float* ko, int ldk, float* vo, int ldv,
                           hipStream_t st) {
     if (n <= 0) return hipSuccess;
-    const int64_t blocks = ((int64_t) n * (c.kv * c.dim / 4) + 255) / 256;
+    // eight tokens a thread from where that still leaves eight workgroups a CU
+    const int64_t pieces = c.kv * c.dim / 4, u = n * pieces >= 8 * 8 * 256 * 256 ? 8 : 1;
+    const int64_t blocks = ((n + u - 1) / u * pieces + 255) / 256;
     if (blocks > INT32_MAX) return hipErrorNotSupported;
     const dim3 grid((uint32_t) blocks, ko != nullptr && vo != nullptr ? 2 : 1);
+    auto go = [&](auto type) {
+        constexpr int T = decltype(type)::value;
+        if (u == 8) kv_read_kernel<T, 8><<<grid, 256, 0, st>>>(c, slots, n, ko, ldk, vo, ldv);
+        else kv_read_kernel<T, 1><<<grid, 256, 0, st>>>(c, slots, n, ko, ldk, vo, ldv);
+    };
     switch (type) {
-        case F16: kv_read_kernel<F16><<<grid, 256, 0, st>>>(c, slots, n, ko, ldk, vo, ldv); break;
-        case Q8_0: kv_read_kernel<Q8_0><<<grid, 256, 0, st>>>(c, slots, n, ko, ldk, vo, ldv); break;
-        case Q4_0: kv_read_kernel<Q4_0><<<grid, 256, 0, st>>>(c, slots, n, ko, ldk, vo, ldv); break;
+        case F16: go(std::integral_constant<int, F16>{}); break;
+        case Q8_0: go(std::integral_constant<int, Q8_0>{}); break;
+        case Q4_0: go(std::integral_constant<int, Q4_0>{}); break;
         default: return hipErrorNotSupported;
     }
     return hipGetLastError();
