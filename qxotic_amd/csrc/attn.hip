@@ -12,6 +12,7 @@ hipError_t launch_attn_q4(const AttnArgs& a, hipStream_t st);
 
 namespace {
 
+// 2048 rows of 128 in 33 parts, 35 MB: 9.9 us; with each part's load behind the one before 16.6.
 // One output row a wave: its parts (m_i, l_i, o_i) joined as Σ 2^(m_i - M) o_i / Σ 2^(m_i - M) l_i over the parts whose keys it
 // sees any of (no other part was written).
 template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, AttnPlan p) {

@@ -7,6 +7,8 @@
 //
 // A pair is (p, p + rope_dim / 2) or, `neighbours`, (2p, 2p + 1); the elements past rope_dim keep their values.
 // The angle is a product in 64 bits (a position of 10^5 times a frequency near 1 has no fraction left to speak of in 32).
+// Bound by memory at many tokens: 4096 of 64 + 8 heads of 64 34 us (4.4 TB/s, a large copy's 4.76); 2048 of 32 + 8 + 8 heads of 128
+// into Q4_0 28 us (3.1 TB/s; the keys' 64-bit arithmetic and the codes). One token is the launch, 4 us from Python.
 // What is only returned is computed in 32 bits; a key that is rounded to a code is computed in 64 up to the f32 value that
 // the code is taken from, so that its code does not depend on the order of the norm's sum.
 #include "kvcache.h"

@@ -148,6 +148,10 @@ CASES = {
     "more_queries_than_keys": (1, 2, 64, 16, [(10, [(2, 5), (0, 3)])], [(2, 6)], 0, False),
     "group_16": (1, 16, 128, 16, [(130, [(20, 1), (33, 1)])], [(61, 1)], 0, False),
     "group_20": (1, 20, 64, 16, [(130, [(20, 1), (33, 2)])], [(61, 1)], 0, False),
+    "many_sequences": (1, 4, 64, 16, [(200, [(1 + i % 37, 1) for i in range(70)])], [(9, 1)], 0, False),
+    "many_groups": (1, 2, 64, 16, [(130 + j % 9, [(3, 1), (20, 1 + j % 3)]) for j in range(66)], [], 0, False),
+    "many_sequences_prompts": (1, 1, 64, 16, [(140, [(9, 3) for _ in range(40)]), (150, [(30 + i, 30) for i in range(3)])],
+                               [(5, 2) for _ in range(30)], 17, False),
     "page_1": (1, 2, 64, 1, [(33, [(20, 1), (70, 2)])], [], 0, False),
     "page_7": (1, 2, 64, 7, [(133, [(20, 1), (70, 2)])], [(100, 60)], 0, False),
     "page_1000": (1, 2, 64, 1000, [(133, [(20, 1), (70, 2)])], [(1001, 60)], 0, False),

@@ -145,6 +145,16 @@ def test_sample_largest_k(hip):
               top_p=np.array([0.3, 0.9, 0.999, 0.5], np.float32), u=u)
 
 
+def test_sample_many_rows_and_long_ones(hip):
+    """More rows than a pair of launches takes; rows of more slices than a wave has lanes."""
+    r = np.random.default_rng(3)
+    x = (r.standard_normal((300, 133)) * 2).astype(np.float32)
+    check(hip, x, **params(300, 8, "mixed"))
+    x = (r.standard_normal((3, 300007)) * 2).astype(np.float32)
+    for which in ("none", "all", "top_p"):
+        check(hip, x, **params(3, 9, which))
+
+
 def test_refusals(hip):
     from qxotic_amd.jam import JAM, Sampling
     P, ok = 1 << 20, Sampling(u=1 << 20)
