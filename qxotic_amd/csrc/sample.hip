@@ -732,8 +732,8 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
     }
     // The groups that reach `bound`, then their elements, four a thread and load: those not below lo nor (lo < hi) from hi on.
     // From where half the groups reach it the row is read as it lies. How many;
-    // more than LIST are not kept. [start, start + count): bit patterns outside which none is (0 as +0)
-    auto gather = [&](uint32_t bound, float lo, float hi, uint32_t start, uint32_t count) -> int {
+    // more than LIST are not kept
+    auto gather = [&](uint32_t bound, float lo, float hi) -> int {
         unsigned long long hits = 0;
 #pragma unroll
         for (int i = 0; i < PER; i++)
@@ -750,24 +750,13 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
         __syncthreads();
         uint32_t* const list = reinterpret_cast<uint32_t*>(sh.w) + wave * WAVE_LIST;
         int got = 0;
-        constexpr int WIDE = 8;   // loads in flight
         if (some) {
-            for (int e0 = 0; e0 < 4 * held; e0 += SM_THREADS * WIDE) {
-                float4_t v[WIDE];
-                int at[WIDE];
-#pragma unroll
-                for (int k = 0; k < WIDE; k++) {
-                    const int e = e0 + SM_THREADS * k + tid, p = sh.pass[min(e / 4, held - 1)];
-                    at[k] = e < 4 * held ? p / GROUPS * SLICE + 4 * (p % GROUPS) + 1024 * (e % 4) : n;
-                }
-#pragma unroll
-                for (int k = 0; k < WIDE; k++) v[k] = load4<VEC>(x, at[k], n);
-#pragma unroll
-                for (int k = 0; k < WIDE; k++) {
-                    if (e0 + SM_THREADS * k >= 4 * held) break;   // the same for all
-                    row_end(v[k], x, at[k], n);
-                    collect4(v[k], at[k], lo, hi, list, &got);
-                }
+            for (int e0 = 0; e0 < 4 * held; e0 += SM_THREADS) {
+                const int e = e0 + tid, p = sh.pass[min(e / 4, held - 1)];
+                const int at = e < 4 * held ? p / GROUPS * SLICE + 4 * (p % GROUPS) + 1024 * (e % 4) : n;
+                float4_t v = load4<VEC>(x, at, n);
+                row_end(v, x, at, n);
+                collect4(v, at, lo, hi, list, &got);
             }
         } else {
             for (int i0 = 0; i0 < n; i0 += 4 * 16 * SM_THREADS) {   // 16 loads in flight
@@ -778,10 +767,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
                 for (int k = 0; k < 16; k++) {
                     const int at = i0 + 4 * (SM_THREADS * k + tid);
                     row_end(v[k], x, at, n);
-                    uint32_t near = ~0u;   // one test for four: most hold none
-#pragma unroll
-                    for (int c = 0; c < 4; c++) near = min(near, __builtin_bit_cast(uint32_t, v[k][c] + 0.0f) - start);
-                    if (__any(near < count)) collect4(v[k], at, lo, hi, list, &got);
+                    collect4(v[k], at, lo, hi, list, &got);
                 }
             }
         }
@@ -842,7 +828,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
         __syncthreads();
         bound = bin_first(sh.bin);
         bound = max(bound, key_of(-__builtin_inff()));   // 0 stands for no element
-        found = gather(bound, of_key(bound), __builtin_nanf(""), 0, ~0u);
+        found = gather(bound, of_key(bound), __builtin_nanf(""));
     } else {
         // slices' weights are relative to their own largest
         if (tid < S) sh.factor[tid] = weight(top, of_key(sh.key[tid]), inv_t, sh.pow), sh.bound[tid] = 0;
@@ -852,7 +838,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
             constexpr int BPT = BINS / SM_THREADS;   // a thread's bins, in a row, from the largest values down: last, last - 1, ..
             const int last = BINS - 1 - BPT * tid;
             double s[BPT] = {};
-#pragma unroll 16
+#pragma unroll 8
             for (int i = 0; i < S; i++) {
                 const double f = sh.factor[i];
                 const ulong2 u = *reinterpret_cast<const ulong2*>(hist + i * BINS + last - 3), v = *reinterpret_cast<const ulong2*>(hist + i * BINS + last - 1);
@@ -889,8 +875,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
                 if (last - k == bin) sh.above = above;
                 above = s[k];
             }
-            const uint32_t k0 = max(bin_first(bin), key_of(-__builtin_inff())), k1 = bin + 1 < BINS ? bin_first(bin + 1) : key_of(__builtin_inff()) + 1;
-            found = gather(k0, of_key(k0), bin + 1 < BINS ? of_key(k1) : __builtin_nanf(""), bin >= BINS / 2 ? k0 ^ 0x80000000u : ~(k1 - 1), k1 - k0);
+            found = gather(bin_first(bin), bin ? of_key(bin_first(bin)) : -__builtin_inff(), bin + 1 < BINS ? of_key(bin_first(bin + 1)) : __builtin_nanf(""));
             above = sh.above;
         }
     }
