@@ -567,16 +567,20 @@ JAMHIP_DEV unsigned long long pair_of(uint32_t key, int idx) { return (unsigned 
 JAMHIP_DEV uint32_t pair_key(unsigned long long p) { return (uint32_t) (p >> 32); }
 JAMHIP_DEV int pair_idx(unsigned long long p) { return (int) ~(uint32_t) p; }
 
-// The indices of those of the elements v, from index i on, that are not below lo nor (lo < hi) from hi on, onto the wave's list of
-// `held` so far (each wave has its own, so that none waits for another's count). Whole waves.
+JAMHIP_DEV int wave_below(unsigned long long lanes) {   // how many of them are below this one
+    return (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) lanes, 0));
+}
+
+// The indices of those of the elements v, from index i on, that lie in [lo, hi] (NaN does not), onto the wave's list of `held` so far (each wave has its own, so that none waits for another's count). Whole waves.
 constexpr int WAVE_LIST = 2 * LIST / SM_WAVES;
 JAMHIP_DEV void collect4(const float4_t& v, int i, float lo, float hi, uint32_t* list, int* held) {
 #pragma unroll
     for (int c = 0; c < 4; c++) {
-        const unsigned long long hit = __ballot(v[c] >= lo && !(v[c] >= hi));
+        const bool in = __builtin_amdgcn_fmed3f(v[c], lo, hi) == v[c];
+        const unsigned long long hit = __ballot(in);
         if (!hit) continue;
-        const int k = *held + (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) hit, 0));
-        if (v[c] >= lo && !(v[c] >= hi) && k < WAVE_LIST) list[k] = (uint32_t) (i + c);
+        const int k = *held + wave_below(hit);
+        if (in && k < WAVE_LIST) list[k] = (uint32_t) (i + c);
         *held += __popcll(hit);
     }
 }
@@ -730,7 +734,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
 #pragma unroll
         for (int i = 0; i < PER; i++) coarse[i] = max(max(mine[i][0], mine[i][1]), max(mine[i][2], mine[i][3]));
     }
-    // The groups that reach `bound`, then their elements, four a thread and load: those not below lo nor (lo < hi) from hi on.
+    // The groups that reach `bound`, then their elements, four a thread and load: those in [lo, hi].
     // From where half the groups reach it the row is read as it lies. How many;
     // more than LIST are not kept
     auto gather = [&](uint32_t bound, float lo, float hi) -> int {
@@ -764,10 +768,19 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
 #pragma unroll
                 for (int k = 0; k < 16; k++) v[k] = load4<VEC>(x, i0 + 4 * (SM_THREADS * k + tid), n);
 #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const int at = i0 + 4 * (SM_THREADS * k + tid);
-                    row_end(v[k], x, at, n);
-                    collect4(v[k], at, lo, hi, list, &got);
+                for (int k = 0; k < 16; k++) row_end(v[k], x, i0 + 4 * (SM_THREADS * k + tid), n);
+                uint32_t half[2] = {0, 0};   // the thread's 64 elements, the first one's bit at the top
+#pragma unroll
+                for (int e = 0; e < 64; e++) {
+                    const float a = v[e / 4][e % 4];
+                    half[e / 32] = half[e / 32] << 1 | (__builtin_amdgcn_fmed3f(a, lo, hi) == a ? 1u : 0u);
+                }
+                unsigned long long bits = (unsigned long long) half[0] << 32 | half[1];
+                for (unsigned long long some = __ballot(bits != 0); some; some = __ballot(bits != 0)) {   // one of each lane's a round
+                    const int e = __clzll(bits | 1), k = got + wave_below(some);
+                    if (bits && k < WAVE_LIST) list[k] = (uint32_t) (i0 + 4 * (SM_THREADS * (e / 4) + tid) + e % 4);
+                    got += __popcll(some);
+                    if (bits) bits &= ~(1ull << (63 - e));
                 }
             }
         }
@@ -828,7 +841,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
         __syncthreads();
         bound = bin_first(sh.bin);
         bound = max(bound, key_of(-__builtin_inff()));   // 0 stands for no element
-        found = gather(bound, of_key(bound), __builtin_nanf(""));
+        found = gather(bound, of_key(bound), __builtin_inff());
     } else {
         // slices' weights are relative to their own largest
         if (tid < S) sh.factor[tid] = weight(top, of_key(sh.key[tid]), inv_t, sh.pow), sh.bound[tid] = 0;
@@ -875,7 +888,9 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
                 if (last - k == bin) sh.above = above;
                 above = s[k];
             }
-            found = gather(bin_first(bin), bin ? of_key(bin_first(bin)) : -__builtin_inff(), bin + 1 < BINS ? of_key(bin_first(bin + 1)) : __builtin_nanf(""));
+            // its largest value; below the first bin from 0 on that is the one before -0, which is a 0
+            const uint32_t next = bin + 1 < BINS ? bin_first(bin + 1) : key_of(__builtin_inff()) + 1;
+            found = gather(bin_first(bin), bin ? of_key(bin_first(bin)) : -__builtin_inff(), of_key(next - (bin + 1 == BINS / 2 ? 2 : 1)));
             above = sh.above;
         }
     }
