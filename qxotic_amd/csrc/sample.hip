@@ -755,9 +755,27 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
         uint32_t* const list = reinterpret_cast<uint32_t*>(sh.w) + wave * WAVE_LIST;
         int got = 0;
         if (some) {
-            for (int e0 = 0; e0 < 4 * held; e0 += SM_THREADS) {
-                const int e = e0 + tid, p = sh.pass[min(e / 4, held - 1)];
-                const int at = e < 4 * held ? p / GROUPS * SLICE + 4 * (p % GROUPS) + 1024 * (e % 4) : n;
+            auto place = [&](int e) {
+                const int p = sh.pass[min(e / 4, held - 1)];
+                return e < 4 * held ? p / GROUPS * SLICE + 4 * (p % GROUPS) + 1024 * (e % 4) : n;
+            };
+            int e0 = 0;
+            for (; e0 + 4 * SM_THREADS <= 4 * held; e0 += 4 * SM_THREADS) {   // four loads in flight
+                float4_t v[4];
+                int at[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) at[k] = place(e0 + SM_THREADS * k + tid);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = load4<VEC>(x, at[k], n);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    row_end(v[k], x, at[k], n);
+                    collect4(v[k], at[k], lo, hi, list, &got);
+                }
+            }
+#pragma unroll 1
+            for (; e0 < 4 * held; e0 += SM_THREADS) {
+                const int at = place(e0 + tid);
                 float4_t v = load4<VEC>(x, at, n);
                 row_end(v, x, at, n);
                 collect4(v, at, lo, hi, list, &got);
