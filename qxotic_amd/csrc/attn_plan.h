@@ -15,6 +15,8 @@ namespace jamhip {
 constexpr int attn_rows(int cfg) { return cfg == 0 ? 16 : cfg == 1 ? 32 : 128; }
 constexpr int attn_keys(int cfg, int dim) { return cfg < 2 ? 128 : dim > 128 ? 32 : 64; }
 constexpr int ATTN_WIDE_DIM = 192;   // the largest head_dim whose 32 rows fit a wave's registers beside the codes
+// Rows of two 32-row tiles: their own reads of the keys against a 128-row tile half empty, 30.5 / 32.8 us for 36 rows behind 8000
+// tokens in Q8_0, 32.4 / 34.4 for 64, F16 35.8 / 37.6.
 inline int attn_cfg(int64_t rows, int dim) { return rows <= 16 ? 0 : rows <= 64 && dim <= ATTN_WIDE_DIM ? 1 : 2; }
 
 // One launch: `tiles` row tiles and `splits` runs of `chunk` keys of each, whose results go to workspace slots from slot0 on,
@@ -47,8 +49,14 @@ inline int attn_splits(int cfg, int64_t groups, int keys, int longest, int* chun
 inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, int n_prefixes, int max_q, int max_seq, int max_prefix) {
     AttnPlan p{};
     const int64_t rows = (int64_t) max_q * grp;
-    // A prefix is worth reading once for its group while one sequence's rows leave a tile partly empty, and something is shared.
-    const bool grouped = n_prefixes > 0 && n_seqs > n_prefixes && rows < attn_rows(2) && max_prefix > 128;
+    // A prefix read once for its group costs a second launch, the joining of every sequence and emptier tiles, 8 us for 16 sequences
+    // and 16 for 64; what it saves grows with the keys that the group's other sequences do not walk again, less where a sequence's
+    // own rows fill a 16-row tile, since their products stay. In us, grouped against sequence by sequence, Q8_0, heads of 128, 8 key
+    // heads and 4 rows unless said: 64 sequences behind 400 tokens 32 / 20, 800 32 / 27, 2000 34 / 49; 16 behind 800 22 / 16, 2000
+    // 24 / 24; 4 behind 6000 25 / 19; 64 behind 2000 with 2 key heads 28 / 24, with 1 27 / 19, of 16 rows 60 / 50; 16 of 32 rows
+    // behind 3000 45 / 35, 16000 95 / 105; 64 of 32 rows behind 4000 109 / 101, 16000 288 / 357.
+    const int64_t saved = (n_seqs - 4 * (int64_t) n_prefixes) * kv * max_prefix, cost = (60000 + 7500 * (int64_t) n_seqs) * (rows <= 8 ? 1 : 4);
+    const bool grouped = n_prefixes > 0 && rows < attn_rows(2) && saved >= cost;
     auto add = [&](int mode, int cfg, int64_t tiles, int64_t busy, int longest) {   // busy: tiles with rows
         AttnPart& a = p.part[p.n++];
         a.mode = mode, a.cfg = cfg, a.tiles = (int) tiles, a.slot0 = p.slots;

@@ -92,6 +92,8 @@ def test_choices(lib):
     modes = lambda *a: [(p["mode"], p["cfg"]) for p in plan(lib, *a)[1]]   # noqa: E731
     assert modes(128, 8, 4, 64, 64, 1, 1, 1024, 8192) == [(1, 2), (2, 0)]
     assert modes(128, 8, 4, 32, 32, 4, 1, 300, 24001) == [(1, 1), (2, 0)]
+    assert modes(128, 8, 4, 16, 16, 1, 1, 200, 4000) == [(1, 1), (2, 0)] and modes(128, 8, 4, 16, 16, 1, 1, 200, 1500) == [(0, 0)]
+    assert modes(128, 8, 4, 512, 64, 1, 8, 100, 16000) == [(1, 2), (2, 1)] and modes(128, 8, 4, 512, 64, 1, 8, 100, 2000) == [(0, 1)]
     assert modes(128, 8, 4, 1, 1, 1, 1, 45, 700) == [(0, 0)]
     assert modes(64, 8, 8, 1792, 8, 1, 256, 256, 4096) == [(0, 2)]
     assert modes(128, 8, 4, 64, 64, 1, 1, 1024, 100) == [(0, 0)]

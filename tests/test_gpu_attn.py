@@ -152,6 +152,16 @@ CASES = {
     "many_groups": (1, 2, 64, 16, [(130 + j % 9, [(3, 1), (20, 1 + j % 3)]) for j in range(66)], [], 0, False),
     "many_sequences_prompts": (1, 1, 64, 16, [(140, [(9, 3) for _ in range(40)]), (150, [(30 + i, 30) for i in range(3)])],
                                [(5, 2) for _ in range(30)], 17, False),
+    # prefixes that are read once for their group: 128-, 32- and 16-row tiles, groups beyond a wave's lanes
+    "grouped_128": (8, 4, 64, 16, [(1301, [(1 + 3 * i, 1) for i in range(40)])], [(9, 1)], 0, False),
+    "grouped_128_dim_128": (8, 4, 128, 16, [(1300, [(1 + 2 * i, 1) for i in range(40)])], [], 0, True),
+    "grouped_32": (8, 3, 64, 16, [(2000, [(3 + i, 1) for i in range(20)]), (1931, [(1 + i, 1) for i in range(12)])], [], 0, False),
+    "grouped_16": (8, 1, 96, 16, [(4100, [(1 + i, 1) for i in range(15)])], [], 0, False),
+    "grouped_window": (8, 2, 64, 16, [(1500, [(1 + 60 * i, 1) for i in range(36)])], [], 1000, True),
+    "grouped_tokens": (8, 2, 64, 64, [(1400, [(3 + i, 1 + i % 4) for i in range(38)])], [(30, 4)], 0, False),
+    "grouped_many": (8, 2, 64, 16, [(1950 - j % 5, [(1 + (i + j) % 20, 1) for i in range(8)]) for j in range(67)], [(7, 1)], 0, False),
+    "grouped_256": (8, 1, 256, 16, [(2300, [(1 + i, 1) for i in range(24)])], [], 0, False),
+    "grouped_192": (8, 2, 192, 16, [(2300, [(1 + i, 1) for i in range(24)])], [], 0, False),
     "page_1": (1, 2, 64, 1, [(33, [(20, 1), (70, 2)])], [], 0, False),
     "page_7": (1, 2, 64, 7, [(133, [(20, 1), (70, 2)])], [(100, 60)], 0, False),
     "page_1000": (1, 2, 64, 1000, [(133, [(20, 1), (70, 2)])], [(1001, 60)], 0, False),
@@ -183,7 +193,8 @@ def test_attn_strides_and_growing_scores(hip, name):
 
 
 @pytest.mark.parametrize("value", [np.nan, np.inf])
-@pytest.mark.parametrize("name", ["one_sequence", "decode_shared", "decode_window", "few_tokens_window", "prompt", "prompt_64", "decode_256"])
+@pytest.mark.parametrize("name", ["one_sequence", "decode_shared", "decode_window", "few_tokens_window", "prompt", "prompt_64", "decode_256",
+                                  "grouped_128", "grouped_16", "grouped_window", "grouped_tokens"])
 def test_attn_masked_entries_change_nothing(hip, name, value):
     """Every entry that no query sees holds NaN or Inf: what lies past the lengths in a page, and, with queries in the middle of a
     prompt, keys and values that later ones see. Rows that do see such an entry are not looked at."""
@@ -279,7 +290,7 @@ def test_attn_long_offsets(hip):
         assert (np.abs(got[4 * h:4 * h + 4] - want[0]) <= (big * (2.0 ** -18 * mass + 2.0 ** -19))[0][:, None]).all()
 
 
-@pytest.mark.parametrize("name", ["decode_shared", "one_sequence", "prompt"])
+@pytest.mark.parametrize("name", ["decode_shared", "one_sequence", "prompt", "grouped_32"])
 def test_attn_in_a_graph_and_on_another_stream(hip, name):
     """Captured once, replayed with other queries and after larger eager calls of the same context: the eager results' bits."""
     import torch
