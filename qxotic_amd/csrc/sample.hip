@@ -16,8 +16,8 @@
 // Weights are summed in histograms as 64-bit integers, so that the order of the atomics does not matter.
 //
 // 128256 logits, first + second launch: one row with all filters 4 + 10 us, without any 6.5 + 7; 64 rows 10 + 13 and 19 + 8 (33 MB: the
-// first is 3.2 TB/s without 64-bit weights, which are the rest). With top-p or min-p alone 64 rows take 27 + 60: where the cut
-// lies in the bulk of the row, its workgroup reads the row again, at what one CU gets from beyond its L2.
+// first is 3.2 TB/s without 64-bit weights, which are the rest). With top-p alone 64 rows take 27 + 44, min-p alone 24 + 30: where the
+// cut lies in the bulk of the row, its workgroup reads the row again, at what one CU gets from beyond its L2.
 #include "launch.h"
 
 namespace jamhip {
@@ -301,7 +301,7 @@ JAMHIP_DEV int sample_general(const Sample& g, int row, uint32_t bk, const RowPa
 }
 
 constexpr int SLICE = 4096, SLICE_THREADS = 256, MAX_SLICES = 64;
-constexpr int BINS = 1024, LIST = SLICE, NARROW = 3072;
+constexpr int BINS = 1024, LIST = SLICE, NARROW = 3000;
 constexpr int GROUPS = SLICE_THREADS;   // 16-element groups of a slice: thread t's, elements 4t + 1024j + {0 .. 3}
 
 // Bins in the order of values: 32 to a power of two from 2^-8 to 2^8, for both signs.
