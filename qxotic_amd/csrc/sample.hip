@@ -19,14 +19,11 @@
 // first is 3.2 TB/s without 64-bit weights, which are the rest). With top-p alone 64 rows take 27 + 44, min-p alone 24 + 30: where the
 // cut lies in the bulk of the row, its workgroup reads the row again, at what one CU gets from beyond its L2.
 #include "launch.h"
+#include "sample_sort.h"
 
 namespace jamhip {
 
 namespace {
-
-// The second launch is a chain of short steps: four waves, one a SIMD, take it at half the time of sixteen, which all repeat
-// what each step does for its wave.
-constexpr int SM_THREADS = 256, SM_WAVES = SM_THREADS / 64;
 
 // A larger value has the larger key; NaN counts as -Inf. Both zeros have one key, as they are equal.
 JAMHIP_DEV uint32_t key_of(float x) {
@@ -535,38 +532,6 @@ JAMHIP_DEV double block_scan(double v, double* lds, double* total) {
     return before + dpp_f64<0x138>(s);   // the lane before's (wave_shr:1; 0 into lane 0)
 }
 
-// list[0 .. n) in falling order; above 256 elements the list is filled up to a power of two with zeros.
-JAMHIP_DEV void sort_falling(unsigned long long* list, int n) {
-    const int tid = threadIdx.x;
-    if (n <= SM_THREADS) {   // an element's place is the number of larger ones
-        const unsigned long long v = tid < n ? list[tid] : 0;
-        int place = 0;
-        if (tid < n)
-            for (int i = 0; i < n; i++) place += list[i] > v;
-        __syncthreads();
-        if (tid < n) list[place] = v;
-        __syncthreads();
-        return;
-    }
-    int size = 2 * SM_THREADS;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += SM_THREADS) list[i] = 0;
-    __syncthreads();
-    for (int k = 2; k <= size; k <<= 1)   // a bitonic network
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            for (int p = tid; p < size / 2; p += SM_THREADS) {
-                const int a = 2 * p - (p & (j - 1)), b = a + j;   // bit j of a is 0
-                const unsigned long long u = list[a], v = list[b];
-                if ((u < v) == ((a & k) == 0)) list[a] = v, list[b] = u;
-            }
-            __syncthreads();
-        }
-}
-
-JAMHIP_DEV unsigned long long pair_of(uint32_t key, int idx) { return (unsigned long long) key << 32 | (uint32_t) ~idx; }
-JAMHIP_DEV uint32_t pair_key(unsigned long long p) { return (uint32_t) (p >> 32); }
-JAMHIP_DEV int pair_idx(unsigned long long p) { return (int) ~(uint32_t) p; }
-
 JAMHIP_DEV int wave_below(unsigned long long lanes) {   // how many of them are below this one
     return (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) lanes, 0));
 }
@@ -923,10 +888,7 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
         const int m = kept_of(sh, way == TOP_K ? rp.k : found, top, inv_t, rp, above, goal, way == TOP_K && rp.p < 1.0 ? fmax(rp.p, 1e-300) : 0.0,
                               first);
         if (way == TOP_K) {
-#pragma unroll 1
-            for (int e = tid; e < m; e += SM_THREADS)   // by index, its place in the list beside it
-                sh.list[e] = (sh.list[e] & 0xFFFFFFFFull) << 32 | (unsigned) e;
-            sort_falling(sh.list, m);
+            order_by_index(sh.list, m);
             const int per = (m + SM_THREADS - 1) / SM_THREADS, from = min(m, tid * per), count = min(m, from + per) - from;
             auto of = [&](int i) { return sh.w[(uint32_t) sh.list[from + i]]; };
             double mine_sum = 0.0, total;

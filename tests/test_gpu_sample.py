@@ -145,6 +145,16 @@ def test_sample_largest_k(hip):
               top_p=np.array([0.3, 0.9, 0.999, 0.5], np.float32), u=u)
 
 
+@pytest.mark.parametrize("vocab", [301, 20000, 128256])
+def test_sample_k_of_several_waves(hip, vocab):
+    """top-k alone, of 65 to 256: the kept ones are put into the vocabulary's order by several waves in one pass."""
+    say("sample k of several waves", vocab)
+    r = np.random.default_rng(vocab)
+    k = np.concatenate([[64, 65, 66, 127, 128, 129, 191, 192, 193, 255, 256, 257], r.integers(65, 257, 52)]).astype(np.int32)
+    x = r.standard_normal((k.size, vocab)).astype(np.float32)
+    check(hip, x, temperature=np.full(k.size, 3.0, np.float32), top_k=k, u=(r.random(k.size) * (1 - 2.0 ** -24)).astype(np.float32))
+
+
 def test_sample_many_rows_and_long_ones(hip):
     """More rows than a pair of launches takes; rows of more slices than a wave has lanes."""
     r = np.random.default_rng(3)
