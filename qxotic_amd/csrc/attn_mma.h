@@ -5,10 +5,11 @@
 //   Oᵀ = Vᵀ · Pᵀ           the scores' registers are the second operand's as they stand: its slots take the keys in the order in
 //                          which the first product leaves them, and Vᵀ comes out of row-major shared memory in that order
 //                          through the transposing read
-// What a code stands for is an f16, so keys and values lose nothing. Queries and weights are f32 values carried as two f16, hi + lo
-// (22 bits), a product each; the query row is scaled by a power of two to a largest element in [1, 2), and weights are
-// 2^(s - m + 7), so neither half runs out of range or into f16's last bits. The running maximum m moves only when a score
-// passes it by 8 (in powers of two; weights then stay below 2^15), so most tiles rescale nothing. Sums are f32.
+// What a code stands for is an f16, so keys and values lose nothing. Queries and weights are f32 values carried as two f16, hi + lo,
+// both cut toward zero (22 bits, 2^-21 of the value at most), a product each. An f16 ends at 2^-24, so the query row is scaled by a power
+// of two to a largest element in [2^14, 2^15), near f16's own: elements down to 2^-17 of it keep their 22 bits, smaller ones are off
+// by at most 2^-38 of it. Weights are 2^(s - m + 7). The running maximum m moves only when a score passes it by 8 (in powers of two;
+// weights then stay below 2^15), so most tiles rescale nothing. Sums are f32.
 #pragma once
 
 #include "attn.h"
@@ -97,7 +98,7 @@ template <int NC, int STEPS, typename AT> JAMHIP_DEV float load_query(const floa
         for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[st][i]));
     }
     top = column_max<NC>(top);
-    const int e = max(top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0, -126);
+    const int e = max((top > 0.0f && top < __builtin_inff() ? ilogbf(top) : 0) - 14, -126);
     const float unit = ldexpf(1.0f, -e);
 #pragma unroll
     for (int st = 0; st < STEPS; st++)
