@@ -6,10 +6,12 @@
 //                          which the first product leaves them, and Vᵀ comes out of row-major shared memory in that order
 //                          through the transposing read
 // What a code stands for is an f16, so keys and values lose nothing. Queries and weights are f32 values carried as two f16, hi + lo,
-// both cut toward zero (22 bits, 2^-21 of the value at most), a product each. An f16 ends at 2^-24, so the query row is scaled by a power
-// of two to a largest element in [2^14, 2^15), near f16's own: elements down to 2^-17 of it keep their 22 bits, smaller ones are off
-// by at most 2^-38 of it. Weights are 2^(s - m + 7). The running maximum m moves only when a score passes it by 8 (in powers of two;
-// weights then stay below 2^15), so most tiles rescale nothing. Sums are f32.
+// both cut toward zero (22 bits, 2^-21 of the value at most), a product each. An f16 ends at 2^-24, so both are scaled to near its other
+// end: the query row by a power of two to a largest element in [2^14, 2^15), of which elements down to 2^-17 keep their 22 bits and
+// smaller ones are off by at most 2^-38; weights are 2^(s - m + 13), which keep them down to 2^-16 of the running maximum m's and
+// are off by at most 2^-37 of it below. m moves only when a score passes it by 2.75 (in powers of two; weights then stay below 2^15.75),
+// so most tiles rescale nothing: against 2^(s - m + 7) and a lag of 8, 64 sequences behind 8192 tokens in Q8_0 take 71.6 us for
+// 70.5, prompts the same. Sums are f32; the matrix cores round each product at about 2^-27 of the sum that it joins.
 #pragma once
 
 #include "attn.h"
@@ -28,7 +30,7 @@ struct AttnArgs {
     float2* ml;    // [slot][token · heads + head]: maximum (powers of two), sum (times 2^WEIGHT_EXP)
 };
 
-constexpr float WEIGHT_EXP = 7.0f, LAZY = 8.0f, LOG2E = 1.44269504088896340736f;
+constexpr float WEIGHT_EXP = 13.0f, LAZY = 2.75f, LOG2E = 1.44269504088896340736f;
 
 template <int TYPE> constexpr int unit_elems() { return TYPE == F16 ? 8 : TYPE == Q8_0 ? 16 : 32; }   // of 16 bytes of codes
 
