@@ -366,8 +366,8 @@ typedef struct {
  * cache's kv_heads; consecutive heads share a key head); with window > 0 only the last `window` of them. sinks: f32 [q_heads]
  * logits that count in the softmax's sum and have no value, or NULL. A row that sees no key is zeros. q [n_tokens][ldq] and out
  * [n_tokens][ldo] are f32 and do not overlap. What a masked entry holds, NaN and Inf included, changes nothing. A shared prefix
- * is read once for its group where that is less work (few query tokens a sequence). head_dim 64, 96, 128, 192 or 256 (else
- * JAMHIP_EUNSUPPORTED). */
+ * is read once for its group where that is less work (few query tokens a sequence). head_dim 64, 96, 128, 192 or 256, and
+ * n_seqs * (max_q * q_heads / 128 + cache's kv_heads) below 2^30 (else JAMHIP_EUNSUPPORTED). */
 jamhip_status jamhip_attn_shared_prefix(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const jamhip_attn_batch* batch,
                                         const void* q_dev, int ldq, int q_heads, float scale, int window, const void* sinks_dev,
                                         void* out_dev, int ldo);

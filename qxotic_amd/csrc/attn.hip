@@ -19,7 +19,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
     __shared__ float redo[4][ATTN_ROW_FLOATS];
     const Attn& g = a.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t n = (int64_t) g.n_tokens * g.heads, i = (int64_t) blockIdx.x * 4 + wave;
+    const int64_t n = (int64_t) g.n_tokens * g.heads, i = (a.block0 + (int64_t) blockIdx.x) * 4 + wave;
     if (i >= n) return;
     const int t = (int) (i / g.heads), head = (int) (i - (int64_t) t * g.heads);
     const bool small = fits_lanes(g);
@@ -93,16 +93,17 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
 }
 
 template <int TYPE> hipError_t launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
-    const uint32_t blocks = (uint32_t) (((int64_t) a.g.n_tokens * a.g.heads + 3) / 4);
-    switch (a.g.cache.dim) {
-        case 64: attn_join_kernel<TYPE, 64><<<blocks, 256, 0, st>>>(a, p); break;
-        case 96: attn_join_kernel<TYPE, 96><<<blocks, 256, 0, st>>>(a, p); break;
-        case 128: attn_join_kernel<TYPE, 128><<<blocks, 256, 0, st>>>(a, p); break;
-        case 192: attn_join_kernel<TYPE, 192><<<blocks, 256, 0, st>>>(a, p); break;
-        case 256: attn_join_kernel<TYPE, 256><<<blocks, 256, 0, st>>>(a, p); break;
-        default: return hipErrorNotSupported;
-    }
-    return hipGetLastError();
+    return attn_runs(a, ((int64_t) a.g.n_tokens * a.g.heads + 3) / 4, [&](const AttnArgs& a, uint32_t blocks) {
+        switch (a.g.cache.dim) {
+            case 64: attn_join_kernel<TYPE, 64><<<blocks, 256, 0, st>>>(a, p); break;
+            case 96: attn_join_kernel<TYPE, 96><<<blocks, 256, 0, st>>>(a, p); break;
+            case 128: attn_join_kernel<TYPE, 128><<<blocks, 256, 0, st>>>(a, p); break;
+            case 192: attn_join_kernel<TYPE, 192><<<blocks, 256, 0, st>>>(a, p); break;
+            case 256: attn_join_kernel<TYPE, 256><<<blocks, 256, 0, st>>>(a, p); break;
+            default: return hipErrorNotSupported;
+        }
+        return hipGetLastError();
+    });
 }
 
 AttnPlan plan_of(const Attn& g) {
@@ -119,7 +120,8 @@ size_t attn_workspace(const Attn& g) {
 hipError_t launch_attn(int type, const Attn& g, void* work, hipStream_t st) {
     if (g.n_tokens <= 0 || g.n_seqs <= 0) return hipSuccess;
     const AttnPlan p = plan_of(g);
-    AttnArgs a;
+    if (p.n == 0) return hipErrorNotSupported;
+    AttnArgs a{};
     a.g = g;
     a.acc = static_cast<float*>(work);
     a.ml = reinterpret_cast<float2*>(a.acc + (size_t) p.slots * g.n_tokens * g.heads * g.cache.dim);

@@ -7,17 +7,17 @@
 namespace jamhip {
 
 template <int TYPE, int D> hipError_t launch_attn_part(const AttnArgs& a, hipStream_t st) {
-    const int64_t blocks = (int64_t) a.g.cache.kv * a.part.tiles * a.part.splits;
-    if (blocks > INT32_MAX) return hipErrorNotSupported;
-    switch (a.part.cfg) {
-        case 0: attn_wave_kernel<TYPE, D, 16><<<(uint32_t) blocks, 256, 0, st>>>(a); break;
-        case 1:
-            if constexpr (D <= ATTN_WIDE_DIM) attn_wave_kernel<TYPE, D, 32><<<(uint32_t) blocks, 256, 0, st>>>(a);
-            else return hipErrorNotSupported;   // attn_cfg does not choose it
-            break;
-        default: attn_tile_kernel<TYPE, D><<<(uint32_t) blocks, 256, 0, st>>>(a); break;
-    }
-    return hipGetLastError();
+    return attn_runs(a, (int64_t) a.g.cache.kv * a.part.tiles * a.part.splits, [&](const AttnArgs& a, uint32_t blocks) {
+        switch (a.part.cfg) {
+            case 0: attn_wave_kernel<TYPE, D, 16><<<blocks, 256, 0, st>>>(a); break;
+            case 1:
+                if constexpr (D <= ATTN_WIDE_DIM) attn_wave_kernel<TYPE, D, 32><<<blocks, 256, 0, st>>>(a);
+                else return hipErrorNotSupported;   // attn_cfg does not choose it
+                break;
+            default: attn_tile_kernel<TYPE, D><<<blocks, 256, 0, st>>>(a); break;
+        }
+        return hipGetLastError();
+    });
 }
 
 template <int TYPE> hipError_t launch_attn_part(const AttnArgs& a, hipStream_t st) {

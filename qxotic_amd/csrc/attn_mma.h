@@ -28,7 +28,18 @@ struct AttnArgs {
     AttnPart part;
     float* acc;    // [slot][token · heads + head][dim], unscaled
     float2* ml;    // [slot][token · heads + head]: maximum (powers of two), sum (times 2^WEIGHT_EXP)
+    int block0;    // workgroups of the launches before
 };
+
+// All `blocks` workgroups in runs of ATTN_RUN.
+template <typename F> hipError_t attn_runs(AttnArgs a, int64_t blocks, F&& launch) {
+    hipError_t e = hipSuccess;
+    for (int64_t b = 0; b < blocks && e == hipSuccess; b += ATTN_RUN) {
+        a.block0 = (int) b;
+        e = launch(a, (uint32_t) (blocks - b < ATTN_RUN ? blocks - b : ATTN_RUN));
+    }
+    return e;
+}
 
 constexpr float WEIGHT_EXP = 13.0f, LAZY = 2.75f, LOG2E = 1.44269504088896340736f;
 

@@ -27,8 +27,11 @@ struct AttnPart {
     bool direct;
 };
 
+// HIP takes fewer than 2^32 threads a launch: a part's workgroups, of 256 each, go out in runs of at most this many.
+constexpr int64_t ATTN_RUN = 1 << 23;
+
 struct AttnPlan {
-    int n;          // launches
+    int n;          // launches; 0: more workgroups than are numbered in 32 bits
     AttnPart part[2];
     int slots;      // workspace results per output row
 };
@@ -48,6 +51,7 @@ inline int attn_splits(int cfg, int64_t groups, int keys, int longest, int* chun
 
 inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, int n_prefixes, int max_q, int max_seq, int max_prefix) {
     AttnPlan p{};
+    bool fits = true;
     const int64_t rows = (int64_t) max_q * grp;
     // A prefix read once for its group costs a second launch, the joining of every sequence and emptier tiles, 8 us for 16 sequences
     // and 16 for 64; what it saves grows with the keys that the group's other sequences do not walk again, less where a sequence's
@@ -62,19 +66,20 @@ inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, in
         a.mode = mode, a.cfg = cfg, a.tiles = (int) tiles, a.slot0 = p.slots;
         a.splits = attn_splits(cfg, busy * kv, attn_keys(cfg, dim), longest, &a.chunk);
         p.slots += a.splits;
+        fits = fits && tiles <= INT32_MAX / kv / a.splits;
     };
     const int cfg = attn_cfg(rows, dim);
     const int64_t per = (rows + attn_rows(cfg) - 1) / attn_rows(cfg);
     if (!grouped) {
         add(0, cfg, per * n_seqs, per * n_seqs, max_seq + max_prefix);
         if (p.slots == 1) p.part[0].direct = true, p.slots = 0;
-        return p;
+        return fits ? p : AttnPlan{};
     }
     const int64_t all = (int64_t) n_tokens * grp;
     const int gcfg = attn_cfg((all + n_prefixes - 1) / n_prefixes, dim), r = attn_rows(gcfg);
     add(1, gcfg, all / r + n_prefixes, ((all + n_prefixes - 1) / n_prefixes + r - 1) / r * n_prefixes, max_prefix);
     add(2, cfg, per * n_seqs, per * n_seqs, max_seq);
-    return p;
+    return fits ? p : AttnPlan{};
 }
 
 }  // namespace jamhip

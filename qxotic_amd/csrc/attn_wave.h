@@ -125,7 +125,7 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
     const Attn& g = a.g;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane % NC, part = lane / NC;
-    int b = blockIdx.x;
+    int b = a.block0 + blockIdx.x;
     const int kvh = b % g.cache.kv;
     b /= g.cache.kv;
     // a prefix's tiles past the last are the last workgroups; a sequence's run of keys past its end is

@@ -99,6 +99,31 @@ def test_choices(lib):
     assert modes(128, 8, 4, 64, 64, 1, 1, 1024, 100) == [(0, 0)]
 
 
+def test_workgroups_past_32_bits(lib):
+    """A call whose workgroups pass 2^31 has no plan; one below keeps every tile. The header's bound is on the safe side."""
+    tiles = lambda *a: [p["tiles"] * p["splits"] for p in plan(lib, *a)[1]]   # noqa: E731
+    assert tiles(128, 8, 8, 34815, 2048, 0, 32768, 32768, 0) == [2048 * 2048]           # 33.5 million workgroups
+    assert tiles(64, 8, 1, 1 << 20, 16383, 0, 1 << 20, 99, 0) == [16383 * 8192]
+    for seqs in (1 << 15, 1 << 16, 1 << 19, 1 << 20, (1 << 20) + 1):                    # cut to 32 bits: negative, 0, 0, 0, 8192
+        assert plan(lib, 64, 8, 1, 1 << 20, seqs, 0, 1 << 20, 99, 0) == (0, [])
+    r = random.Random(3)
+    some = 0
+    for _ in range(4000):
+        dim, kv, grp = r.choice([64, 96, 128, 192, 256]), r.choice([1, 2, 8]), r.choice([1, 4, 7, 16, 20])
+        most = ((1 << 31) - 4097) // (kv * grp)
+        tokens, seqs = int(most ** r.random()), int(2 ** (24 * r.random()))
+        max_q, n = int(tokens ** r.random()), r.choice([0, 1, seqs // 5])
+        _, parts = plan(lib, dim, kv, grp, tokens, seqs, n, max_q, r.choice([1, 129, 1 << 20]), r.choice([1, 5000, 100000]) if n else 0)
+        for p in parts:
+            rows = lib.q_rows(p["cfg"])
+            assert p["tiles"] == (tokens * grp // rows + n if p["mode"] == 1 else seqs * -(-max_q * grp // rows))
+            assert p["tiles"] * p["splits"] * kv < 1 << 31
+        if seqs * (max_q * kv * grp // 128 + kv) < 1 << 30:
+            assert parts
+        some += not parts
+    assert some > 100
+
+
 def test_fast_division(lib):
     r = random.Random(2)
     for d in [1, 2, 3, 5, 7, 16, 24, 100, 1000, 65535, 65536, 65537, (1 << 30) + 1, (1 << 31) - 1] + [r.randint(1, (1 << 31) - 1) for _ in range(50)]:
