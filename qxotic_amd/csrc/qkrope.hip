@@ -67,6 +67,16 @@ template <int LPH> JAMHIP_DEV double head_sum(double v) {
     return v;
 }
 
+// 1 / sqrt(v). In 32 bits with one rounding, as the definition has it (a root and a division have two): the instruction's value r, off
+// by an ulp at most, corrected by half of what v · r² leaves of 1, the product v · r in two parts.
+JAMHIP_DEV double inv_sqrt(double v) { return 1.0 / sqrt(v); }
+JAMHIP_DEV float inv_sqrt(float v) {
+    const float r = rsqrtf(v);
+    if (!(r > 0.0f && r < __builtin_inff())) return r;   // of 0, Inf and NaN
+    const float h = v * r, rest = fmaf(-r, fmaf(v, r, -h), fmaf(-r, h, 1.0f));
+    return fmaf(0.5f * r, rest, r);
+}
+
 // 8 consecutive elements of a row, from element 8·j on, into the cache. Four neighbouring lanes hold one block of 32.
 template <int TYPE> JAMHIP_DEV void cache_store8(const KvView& c, uint8_t* buf, int64_t row, int j, const float* x) {
     if constexpr (TYPE == F16) {
@@ -156,7 +166,7 @@ template <typename T, int LPH, bool VEC> struct Head {
 #pragma unroll
         for (int i = 0; i < 4; i++) ss += a[i] * a[i] + b[i] * b[i];
         ss = head_sum<LPH>(ss);
-        const T r = (T) 1 / sqrt(ss / (T) dim + (T) eps);
+        const T r = inv_sqrt(ss / (T) dim + (T) eps);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int p = pair(i);
