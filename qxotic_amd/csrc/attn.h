@@ -53,7 +53,8 @@ JAMHIP_DEV int seq_of(const Attn& g, int t) {
 }
 
 // A batch of up to 64 sequences and 64 groups in a wave's lanes: one round of loads, where a search through the arrays is a chain
-// of them (a load that misses takes 1 us, a small call's attention 4).
+// of them (a load that misses takes 1 us, a small call's attention 4). 64 and 65 sequences of 500 tokens in Q8_0, 8 key heads of 128:
+// 18.7 and 27.0 us a call, behind a shared prefix of 2000 43 and 56.
 struct BatchLanes {
     int off, next, len;      // of sequence `lane`; next: the end of its query tokens
     int cut, cut_next, plen; // of group `lane`

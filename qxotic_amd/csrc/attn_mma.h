@@ -328,7 +328,7 @@ template <int TYPE, int STRIDE> JAMHIP_DEV void put_unit(uint8_t* plane, const u
         if constexpr (TYPE == Q8_0) {
 #pragma unroll
             for (int i = 0; i < 4; i++) q8_word(w[i], scale, h + 2 * i);
-        } else {   // byte j: element j low, element 16 + j high. An absent key's scale is 0
+        } else {   // byte j: element j low, element 16 + j high
 #pragma unroll
             for (int i = 0; i < 4; i++) q4_word(w[i], scale, h + 2 * i), q4_word(w[i] >> 4, scale, h + 8 + 2 * i);
         }

@@ -30,6 +30,10 @@ struct AttnPart {
 // HIP takes fewer than 2^32 threads a launch: a part's workgroups, of 256 each, go out in runs of at most this many.
 constexpr int64_t ATTN_RUN = 1 << 23;
 
+// Tiles and runs follow the call's maxima, not the device's lengths, so a call fits what it is told and no more. A max_seq_len far above the
+// lengths leaves few workgroups with keys: one sequence of 1000 tokens 11.5 us at 1000, 12.8 at 16384, 23.5 at 131072; of 8000 16.7 at 8000,
+// 43.7 at 131072. A max_q far above most sequences' query tokens gives each mostly empty tiles and its prefix no group: 63 sequences'
+// next tokens and a prompt of 1024, behind 8192 shared tokens, 2030 us in one call, 408 in one for the decoding and one for the prompt.
 struct AttnPlan {
     int n;          // launches; 0: more workgroups than are numbered in 32 bits
     AttnPart part[2];

@@ -7,8 +7,10 @@
 // Bound by the matrix cores and the VALU alike, each busy about half of the time: at head_dim 64 a tile costs a wave 1024 cycles of
 // products (two for each, for the halves) and about 1100 of VALU (an exponential of 16 cycles, a fused multiply-add, a sum, a
 // maximum, two conversions and a difference for each of 32 scores a lane), and two waves a SIMD take 3900 for it. 64 sequences of 4 heads
-// behind 8192 tokens in Q8_0, 8 key heads of 128: 33.6 us; 8 prompts of up to 256 tokens behind 4096 in F16, heads of 64: 292 us (434
-// TFLOP/s, counted once). Two halves of shared memory with one barrier a tile took 37.8 for the first, 16 runs of keys for 32 took 38.
+// behind 8192 tokens in Q8_0, 8 key heads of 128: 31 to 33 us; 8 prompts of up to 256 tokens behind 4096 in F16, heads of 64: 293 to 301 us
+// from card to card (434 to 422 TFLOP/s, counted once) after some fifty calls in a row, 340 to 390 before, while the clock rises. Two halves of
+// shared memory with one barrier a tile took 37.8 for the first, 16 runs of keys for 32 took 38. At head_dim 128 the two halves of
+// the query and the next tile's codes are more than 256 registers: 25 (F16), 14 (Q8_0) and 4 (Q4_0) of them go to scratch, at 256 24 to 33.
 #pragma once
 
 #include "attn_mma.h"

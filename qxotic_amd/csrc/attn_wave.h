@@ -7,9 +7,10 @@
 // read. The next tile's codes are on their way while one is computed.
 //
 // Bound by memory while all workgroups run, then by the longest sequence: 64 sequences of 33 to 1024 keys in Q8_0, 8 key heads of
-// 128, 27 us (2.8 TB/s over all, 6 at the start). With 32 rows behind 4 x 24001 tokens in Q4_0, 48 us (2.3 TB/s), by the VALU, which
-// turns codes into f16 (7 instructions for 4), and the matrix cores. One sequence of 745 keys 7.7 us: launch and three rounds of dependent loads
-// (lengths, pages, codes). A workgroup of one tile with a barrier between loads and products took 28.8 and 76.9 for the first two.
+// 128, 28 to 30 us (2.6 TB/s over all, 6 at the start). With 32 rows behind 4 x 24001 tokens in Q4_0, 51 us (2.1 TB/s): the bytes take about 23
+// of them, the two products 22, turning codes into f16 (7 instructions for 4) 9, and two waves a SIMD do not overlap the three. One
+// sequence of 745 keys 7.1 us: launch and three rounds of dependent loads (lengths, pages, codes). A workgroup of one tile with a barrier
+// between loads and products took 28.8 and 76.9 for the first two. 32 rows of 128 take all registers: 26 (F16) and 2 (Q4_0) go to scratch.
 #pragma once
 
 #include "attn_mma.h"

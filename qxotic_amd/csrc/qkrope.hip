@@ -7,8 +7,11 @@
 //
 // A pair is (p, p + rope_dim / 2) or, `neighbours`, (2p, 2p + 1); the elements past rope_dim keep their values.
 // The angle is a product in 64 bits (a position of 10^5 times a frequency near 1 has no fraction left to speak of in 32).
-// Bound by memory at many tokens: 4096 of 64 + 8 heads of 64 34 us (4.4 TB/s, a large copy's 4.76); 2048 of 32 + 8 + 8 heads of 128
-// into Q4_0 28 us (3.1 TB/s; the keys' 64-bit arithmetic and the codes). One token is the launch, 4 us from Python.
+// Bound by memory at many tokens: 4096 of 64 + 8 heads of 64 34 us (4.4 TB/s, a large copy's 4.76). Into a cache it is bound by latency: no
+// load of a row is issued before the angles are made and the barrier passed, and a key in 64 bits takes 101 to 107 registers (140 for
+// rows that are not 16-byte aligned) where the rotation alone takes 42, so 4 (3) waves a SIMD hide it instead of 8: 2048 tokens of
+// 32 + 8 + 8 heads of 128 into Q4_0 28 us with their rows in the last-level cache, 33 without (3.1 and 2.6 TB/s), 333 of 16 + 2 + 2 of 256 into F16 9.
+// One token is the launch, 4 us from Python.
 // What is only returned is computed in 32 bits; a key that is rounded to a code is computed in 64 up to the f32 value that
 // the code is taken from, so that its code does not depend on the order of the norm's sum.
 #include "kvcache.h"
@@ -323,8 +326,10 @@ template <int TYPE, int U> __global__ void __launch_bounds__(256) kv_read_kernel
 
 template <int TYPE, int LPH> hipError_t launch_rope(QkRope g, bool vec, hipStream_t st) {
     const int all = g.q_heads + g.kv_heads * (TYPE >= 0 ? 2 : 1), at_once = QK_THREADS / LPH;
-    // few tokens: a workgroup per pass of heads, so that no thread does two in a row; many: one per token, whose angles are
-    // then computed once
+    // few tokens: a workgroup per pass of heads, so that no thread does two in a row; many: one per token, whose angles are then
+    // computed once. In us, by pass / by token: 64 + 8 heads of 64, 128 tokens 5.2 / 6.7, 511 7.2 / 9.0, 768 9.7 / 10.6, 1024 12.1 / 11.8;
+    // 32 + 8 of 128, 511 8.7 / 9.8, 768 12.6 / 11.8, 2048 26.7 / 26.0; with 8 more into Q8_0, 64 5.3 / 7.7, 384 9.9 / 10.5, 511 11.8 / 11.2,
+    // 1024 16.8 / 15.7
     g.per = g.n < 512 ? at_once : (all + at_once - 1) / at_once * at_once;
     const dim3 grid(g.n, (all + g.per - 1) / g.per);
     if (vec) qk_norm_rope_kernel<TYPE, LPH, true><<<grid, QK_THREADS, 0, st>>>(g);

@@ -12,11 +12,12 @@
 // candidates to read again and sort; from the histogram the cut falls into one bin, whose elements alone are sorted. The kept
 // set is then {(x, index) >= T}, a slice's kept sum follows from its histogram, and only the slice in which the token lies
 // is read once more. Where candidates or a bin are too many to sort (large k, thousands of equal values), and past 262144
-// logits, the cut is found digit by digit of the values' order-preserving 32-bit keys from histograms over the whole row.
+// logits, the cut is found digit by digit of the values' order-preserving 32-bit keys from histograms over the whole row, by one
+// workgroup: with all filters one row of 262144 takes 15 us and of 262145 2.3 ms, 64 rows 31 us and 4.8 ms.
 // Weights are summed in histograms as 64-bit integers, so that the order of the atomics does not matter.
 //
-// 128256 logits, first + second launch: one row with all filters 4 + 10 us, without any 6.5 + 7; 64 rows 10 + 13 and 19 + 8 (33 MB: the
-// first is 3.2 TB/s without 64-bit weights, which are the rest). With top-p alone 64 rows take 27 + 44, min-p alone 24 + 30: where the
+// 128256 logits, first + second launch: one row with all filters 4 + 10 us, without any 6.5 + 7; 64 rows 11 + 13 and 19 + 7 (33 MB: the
+// first is 3.1 TB/s without 64-bit weights, which are the rest). With top-p alone 64 rows take 26 + 43, min-p alone 23 + 32: where the
 // cut lies in the bulk of the row, its workgroup reads the row again, at what one CU gets from beyond its L2.
 #include "launch.h"
 #include "sample_sort.h"
@@ -536,7 +537,8 @@ JAMHIP_DEV int wave_below(unsigned long long lanes) {   // how many of them are 
     return (int) __builtin_amdgcn_mbcnt_hi((uint32_t) (lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) lanes, 0));
 }
 
-// The indices of those of the elements v, from index i on, that lie in [lo, hi] (NaN does not), onto the wave's list of `held` so far (each wave has its own, so that none waits for another's count). Whole waves.
+// The indices of those of the elements v, from index i on, that lie in [lo, hi] (NaN does not), onto the wave's list of `held` so far
+// (each wave has its own, so that none waits for another's count). Whole waves.
 constexpr int WAVE_LIST = 2 * LIST / SM_WAVES;
 JAMHIP_DEV void collect4(const float4_t& v, int i, float lo, float hi, uint32_t* list, int* held) {
 #pragma unroll
@@ -699,9 +701,8 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
 #pragma unroll
         for (int i = 0; i < PER; i++) coarse[i] = max(max(mine[i][0], mine[i][1]), max(mine[i][2], mine[i][3]));
     }
-    // The groups that reach `bound`, then their elements, four a thread and load: those in [lo, hi].
-    // From where half the groups reach it the row is read as it lies. How many;
-    // more than LIST are not kept
+    // The elements in [lo, hi] onto sh.list, and how many they are; more than LIST are not kept, and LIST + 1 is returned. Where fewer than half
+    // of the groups reach `bound`, their elements alone are read, four a thread and load, else the row as it lies.
     auto gather = [&](uint32_t bound, float lo, float hi) -> int {
         unsigned long long hits = 0;
 #pragma unroll
@@ -793,6 +794,8 @@ template <bool VEC> JAMHIP_DEV int pick_row(const Sample& g, const SampleWork& w
     if (way == TOP_K) {
         // The k-th largest of the largest of every 64 (for large k: 16) elements lies in the bin in which their number, from
         // the top, reaches k: at least k elements are not below that bin's first value
+        // Of every 64 there are S · GROUPS / 4, of which k has to leave the bound well above their smallest: 128256 logits, one row, by 64 /
+        // by 16 in us: k = 50 14.5 / 16.0, 256 27.3 / 28.9, 1024 74.9 / 73.5, 1025 92.9 / 90.6, 2048 741 / 137; 32000: 512 99 / 43
         const bool fine = rp.k > S * GROUPS / 8;
         int* const count = reinterpret_cast<int*>(sh.w);
 #pragma unroll
