@@ -347,9 +347,10 @@ jamhip_status jamhip_kv_read(jamhip_ctx* ctx, const jamhip_kv_cache* cache, cons
  * of its seq_lens[s] own tokens, whose entries are in the cache already, at the pages of row s of seq_pages [n_seqs][ld_seq_pages].
  * Prefix group j, the sequences [prefix_seqs[j], prefix_seqs[j + 1]), has prefix_lens[j] tokens in front of the own ones, at the
  * pages of row j of prefix_pages; a sequence outside every group has none. max_q, max_seq_len and max_prefix_len bound the
- * device lengths (what is longer is cut; query tokens past max_q are not computed), and the work is divided by them: a captured step
- * whose max_seq_len is a capacity far above the lengths is slower for it, and prompts among decoding sequences belong in a call of
- * their own, since max_q holds for every sequence of a call. All arrays are int32. A page outside the cache is read as page 0. */
+ * device lengths (lengths past them are cut; a sequence's query tokens past its first max_q are not computed), and the work is
+ * divided by them: a captured step whose max_seq_len is a capacity far above the lengths is slower for it, and prompts among
+ * decoding sequences belong in a call of their own, since max_q holds for every sequence of a call. All arrays are int32. A page
+ * outside the cache is read as page 0. */
 typedef struct {
     int         n_tokens, n_seqs, n_prefixes;
     int         max_q, max_seq_len, max_prefix_len;

@@ -9,7 +9,8 @@
 namespace jamhip {
 
 struct SeqInfo {
-    int t0, nq;           // its query tokens
+    int t0, nq;           // its query tokens that are computed
+    int first;            // the first one's place among its own tokens
     int base, len;        // tokens of its prefix, and its own
     const int* prefix;    // page rows
     const int* own;
@@ -37,8 +38,10 @@ JAMHIP_DEV int prefix_of(const Attn& g, int s) {   // the sequence's prefix grou
 JAMHIP_DEV SeqInfo seq_info(const Attn& g, int s) {
     SeqInfo r;
     r.t0 = clampi(g.q_offsets[s], 0, g.n_tokens);
-    r.nq = min(clampi(g.q_offsets[s + 1], r.t0, g.n_tokens) - r.t0, g.max_q);
+    const int nq = clampi(g.q_offsets[s + 1], r.t0, g.n_tokens) - r.t0;
+    r.nq = min(nq, g.max_q);
     r.len = clampi(g.seq_lens[s], 0, g.seq_cap);
+    r.first = r.len - nq;
     r.own = g.seq_pages + (int64_t) s * g.ld_seq_pages;
     const int j = prefix_of(g, s);
     r.base = j < 0 ? 0 : clampi(g.prefix_lens[j], 0, g.prefix_cap);
@@ -81,8 +84,10 @@ JAMHIP_DEV int lane_int(int v, int l) { return __builtin_amdgcn_readlane(v, l); 
 JAMHIP_DEV SeqInfo seq_info(const Attn& g, const BatchLanes& b, int s) {   // s the same in every lane
     SeqInfo r;
     r.t0 = lane_int(b.off, s);
-    r.nq = min(lane_int(b.next, s) - r.t0, g.max_q);
+    const int nq = lane_int(b.next, s) - r.t0;
+    r.nq = min(nq, g.max_q);
     r.len = lane_int(b.len, s);
+    r.first = r.len - nq;
     r.own = g.seq_pages + (int64_t) s * g.ld_seq_pages;
     const unsigned long long in = __ballot(b.cut <= s && s < b.cut_next);
     const int j = in ? __ffsll(in) - 1 : 0;
@@ -113,7 +118,7 @@ template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, flo
     if (s < 0) return;
     const SeqInfo r = seq_info(g, s);
     if (t - r.t0 >= r.nq) return;
-    const int pos = r.base + r.len - r.nq + (t - r.t0);
+    const int pos = r.base + r.first + (t - r.t0);
     const int lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(r.base + r.len, pos + 1);
     float* qs = lds;
     float* ps = lds + 256;

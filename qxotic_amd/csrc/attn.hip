@@ -29,7 +29,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
     if (sq < 0) return;
     const SeqInfo s = small ? seq_info(g, lanes, sq) : seq_info(g, sq);
     if (t - s.t0 >= s.nq) return;
-    const int pos = s.base + s.len - s.nq + (t - s.t0), lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(s.base + s.len, pos + 1);
+    const int pos = s.base + s.first + (t - s.t0), lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(s.base + s.len, pos + 1);
     constexpr int E = D > 128 ? 4 : D > 64 ? 2 : 1;   // elements a lane
     float m = -__builtin_inff(), l = 0.0f, o[E];
 #pragma unroll

@@ -202,24 +202,24 @@ JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowSet& w, int r, int kvh
     c.tok = w.t_first + g.grp.div(rr);
     c.head = kvh * g.grp.d + (rr - (c.tok - w.t_first) * g.grp.d);
     c.live = r < w.n_rows;
-    int pos = total - w.s.nq + (c.tok - w.s.t0);
+    int pos = w.s.base + w.s.first + (c.tok - w.s.t0);
     if (a.part.mode == 1) {
         if (fits_lanes(g)) {   // the sequences of the wave's tokens, one after another
             const BatchLanes& b = w.lanes;
-            int len = 0, t0 = 0, nq = -1;
+            int at = 0, t0 = 0, nq = -1;   // at: SeqInfo::first
             const int t0_wave = wave_min(c.tok), t1_wave = wave_max(c.tok);
             unsigned long long on = __ballot(b.off < b.next && b.next > t0_wave && b.off <= t1_wave);
             for (; on; on &= on - 1) {
                 const int q = __ffsll(on) - 1, first = lane_int(b.off, q), end = lane_int(b.next, q);
-                if (c.tok >= first && c.tok < end) t0 = first, nq = min(end - first, g.max_q), len = lane_int(b.len, q);
+                if (c.tok >= first && c.tok < end) t0 = first, nq = min(end - first, g.max_q), at = lane_int(b.len, q) - (end - first);
             }
             c.live = c.live && c.tok - t0 < nq;
-            pos = w.s.base + len - nq + (c.tok - t0);
+            pos = w.s.base + at + (c.tok - t0);
         } else {
             const int q = seq_of(g, c.tok);
             const SeqInfo mine = seq_info(g, max(q, 0));
             c.live = c.live && q >= 0 && c.tok - mine.t0 < mine.nq;
-            pos = mine.base + mine.len - mine.nq + (c.tok - mine.t0);
+            pos = mine.base + mine.first + (c.tok - mine.t0);
         }
     }
     const int c0 = split * a.part.chunk;

@@ -3,6 +3,7 @@ import sys
 
 import numpy as np
 import pytest
+from test_gpu_attn import CASES, Batch
 
 from oracle import decode as D
 
@@ -39,6 +40,24 @@ def test_more_workgroups_than_a_launch_takes(hip):
             want, mass, big = D.attention(q[i].reshape(1, kv, dim)[:, h:h + 1], vals[0][slots, h], vals[1][slots, h], [lens[i] - 1],
                                           np.float64(np.float32(dim ** -0.5)))
             assert (np.abs(got[i, h] - want[0, 0]) <= (big * (2.0 ** -18 * mass + 2.0 ** -19))[0, 0]).all(), (i, h)   # as in test_gpu_attn.py
+
+
+@pytest.mark.parametrize("name,max_q", [("few_tokens", 5), ("few_tokens_window", 7), ("prompt", 60), ("prompt_64", 100), ("many_sequences_prompts", 2),
+                                        ("grouped_tokens", 3), ("grouped_tokens", 1), ("many_groups", 2), ("page_7", 20)])
+def test_query_tokens_past_max_q(hip, name, max_q):
+    """They are not computed; those before them see the keys up to their own place, not a later one's."""
+    kv, grp, dim, page, groups, alone, window, sinks = CASES[name]
+    print("attn past max_q", name, max_q, file=sys.stderr, flush=True)
+    b = Batch(D.Q8_0, kv, grp, dim, page, groups, alone, window, sinks, seed=max_q)
+    assert max(q for _, q in b.seqs) > max_q
+    got = b.run(hip, max_q=max_q)
+    for i, (_, nq) in enumerate(b.seqs):
+        rows = got[b.off[i]:b.off[i + 1]]
+        assert (rows[max_q:] == -5.0).all()
+        for c in range(kv if nq else 0):
+            want, tol = b.want(i, c)
+            g = rows[:max_q, c * grp * dim:(c + 1) * grp * dim].reshape(want[:max_q].shape)
+            assert (np.abs(g - want[:max_q]) <= tol[:max_q]).all(), (i, c)
 
 
 def test_more_workgroups_than_there_can_be(hip):
