@@ -374,6 +374,89 @@ jamhip_status jamhip_attn_shared_prefix(jamhip_ctx* ctx, const jamhip_kv_cache* 
                                         const void* q_dev, int ldq, int q_heads, float scale, int window, const void* sinks_dev,
                                         void* out_dev, int ldo);
 
+/* ---- A step with drafted trees: several guesses of the tokens that come next, looked at by the model in one pass. A step is
+ * jamhip_kv_resize (room for the drafted tokens, their slots), jamhip_tree_masks, then in every layer jamhip_qkv_norm_rope_write and
+ * jamhip_attn_tree, jamhip_sample on every drafted token's logits, jamhip_tree_accept, jamhip_kv_move for all layers at once, and
+ * jamhip_kv_resize again, to the accepted lengths. The lengths, tables and counts stay on the device; a captured step can be replayed. */
+
+/* Page tables and slots. All arrays are int32 device memory; lens_out, held_out and n_free_out may be lens, held and n_free. */
+typedef struct {
+    int         n_seqs, n_tokens;     /* rows of pos and slots: the batch's capacity */
+    int         page_tokens, n_pages; /* the cache's */
+    int         free_cap, ld_seq_pages;
+    const void* lens;         /* [n_seqs] tokens that each sequence holds */
+    const void* targets;      /* [n_seqs] tokens that it is to hold; below zero: none */
+    const void* base;         /* [n_seqs] added to its positions (tokens of a shared prefix), or NULL */
+    const void* held;         /* [n_seqs] pages that it holds: the first entries of its row of seq_pages */
+    const void* n_free;       /* [1] free pages */
+    void*       free_pages;   /* [free_cap] a list, taken from its end */
+    void*       seq_pages;    /* [n_seqs][ld_seq_pages] */
+    void*       lens_out;     /* [n_seqs] */
+    void*       held_out;     /* [n_seqs] */
+    void*       n_free_out;   /* [1] */
+    void*       status;       /* [n_seqs] 0, or 1: refused */
+    void*       q_offsets;    /* [n_seqs + 1] */
+    void*       pos;          /* [n_tokens] */
+    void*       slots;        /* [n_tokens] */
+} jamhip_kv_pages;
+
+/* Every sequence gets ceil(target / page_tokens) pages. First the pages that are too many go back to the free list, from the last sequence
+ * to the first, each one's last page first; then the sequences take theirs off the list's end, in their order. A sequence that does not
+ * fit (the list is empty, its row is full, or its tokens pass n_tokens) is refused, and so is every one behind it that would grow: they
+ * keep their pages and lengths. Giving back what the call before took leaves the list as it was. A sequence's new tokens, max(0,
+ * target - len) of them, are rows q_offsets[s] on of the batch, refused or not (q_offsets stop at n_tokens); row i of them has the
+ * position base + len + i and the slot of its place, -1 where the sequence was refused. Rows behind the last sequence's get slot -1 and
+ * position 0. n_seqs at most 2^20, n_pages * page_tokens below 2^31 (else JAMHIP_EUNSUPPORTED). */
+jamhip_status jamhip_kv_resize(jamhip_ctx* ctx, const jamhip_kv_pages* pages);
+
+/* A batch of trees: sequence s drafted the tokens [q_offsets[s], q_offsets[s + 1]) of n_tokens; parents[t] is the place of token t's parent
+ * among its sequence's, below its own (anything else: none). Token 0 of a sequence is the root of its tree: the token that the step
+ * before picked. A sequence's tokens past its first max_q are not looked at. int32 device memory. */
+typedef struct {
+    int         n_tokens, n_seqs, max_q;
+    const void* q_offsets;   /* [n_seqs + 1], rising */
+    const void* parents;     /* [n_tokens] */
+} jamhip_tree;
+
+/* masks [n_tokens][mask_words], 64-bit words: bit j of row t says that token t sees its sequence's drafted token j, which are itself and its
+ * ancestors. pos (int32 [n_tokens] or NULL) as jamhip_kv_resize wrote it becomes the first token's position plus the depth. Made once for
+ * a step's layers. mask_words * 64 >= max_q. */
+jamhip_status jamhip_tree_masks(jamhip_ctx* ctx, const jamhip_tree* tree, void* masks_dev, int mask_words, void* pos_dev);
+
+/* jamhip_attn_shared_prefix with the batch's query tokens as drafted trees: a token sees its sequence's tokens before the first query
+ * token, and of the query tokens those whose bits are set in its row of masks [n_tokens][mask_words] (8-byte aligned; any bits, those of
+ * later tokens too; one that does not see itself has to say so). With window > 0 it sees the last `window` keys of that list. Bits past
+ * the sequence's tokens are not looked at. mask_words * 64 >= batch's max_q. Everything else as there. */
+jamhip_status jamhip_attn_tree(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const jamhip_attn_batch* batch, const void* masks_dev,
+                               int mask_words, const void* q_dev, int ldq, int q_heads, float scale, int window, const void* sinks_dev,
+                               void* out_dev, int ldo);
+
+/* What jamhip_tree_accept writes; int32 device memory. Rows of tokens of no sequence are left as they were. */
+typedef struct {
+    int         ld_path;     /* the longest path */
+    void*       path;        /* [n_seqs][ld_path] places of the accepted tokens among their sequence's, rising, then -1 */
+    void*       accepted;    /* [n_seqs] their number: at least 1 for a sequence with tokens, if ld_path is */
+    void*       next;        /* [n_seqs] what the model picked at the last of them, -1 for a sequence without tokens */
+    const void* lens;        /* [n_seqs] lengths before the step; NULL without lens_out */
+    void*       lens_out;    /* [n_seqs] lens + accepted, or NULL; may be lens */
+    const void* slots;       /* [n_tokens] the tokens' slots; NULL without move_from */
+    void*       move_from;   /* [n_tokens] or NULL: for jamhip_kv_move with the same q_offsets, the k-th accepted token's slot */
+    void*       move_to;     /* [n_tokens] and the k-th token's; -1 both where nothing moves */
+} jamhip_tree_path;
+
+/* The drafted tokens that the model agrees with: from token 0 of each sequence on, the first child (the lowest) whose token is what was picked
+ * at its parent, until there is none. tokens, picked: int32 [n_tokens], the drafted tokens and what the model picks after each. With
+ * picks that are samples of the model's own distribution, so are the accepted tokens. */
+jamhip_status jamhip_tree_accept(jamhip_ctx* ctx, const jamhip_tree* tree, const void* tokens_dev, const void* picked_dev,
+                                 const jamhip_tree_path* path);
+
+/* Entry i, keys and values, goes from slot from[i] to slot to[i] (int32 [n]) in each of n_caches caches of one shape. Group j is the entries
+ * [offsets[j], offsets[j + 1]); those of a group are moved in their order, groups at once: a slot that one group writes belongs to no
+ * other. An entry with a slot outside the cache is left out. n_groups at most 2^20 and n_groups * n_caches below 2^31 (else
+ * JAMHIP_EUNSUPPORTED). */
+jamhip_status jamhip_kv_move(jamhip_ctx* ctx, const jamhip_kv_cache* caches, int n_caches, const void* offsets_dev, int n_groups,
+                             const void* from_dev, const void* to_dev, int n);
+
 /* Per-row sampling parameters, device arrays of `rows` entries. NULL: temperature 1, no filter. */
 typedef struct {
     const void* temperature;   /* f32; not above 0: the first of the largest logits */

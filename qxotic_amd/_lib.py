@@ -35,6 +35,27 @@ class AttnBatch(C.Structure):
                 ("prefix_lens", _VP), ("prefix_pages", _VP), ("ld_prefix_pages", _I)]
 
 
+class KvPages(C.Structure):
+    """Page tables and slots of a batch (jamhip_kv_pages); the arrays are device addresses of int32."""
+
+    _fields_ = [("n_seqs", _I), ("n_tokens", _I), ("page_tokens", _I), ("n_pages", _I), ("free_cap", _I), ("ld_seq_pages", _I), ("lens", _VP),
+                ("targets", _VP), ("base", _VP), ("held", _VP), ("n_free", _VP), ("free_pages", _VP), ("seq_pages", _VP), ("lens_out", _VP),
+                ("held_out", _VP), ("n_free_out", _VP), ("status", _VP), ("q_offsets", _VP), ("pos", _VP), ("slots", _VP)]
+
+
+class Tree(C.Structure):
+    """Drafted trees of a batch (jamhip_tree); the arrays are device addresses of int32."""
+
+    _fields_ = [("n_tokens", _I), ("n_seqs", _I), ("max_q", _I), ("q_offsets", _VP), ("parents", _VP)]
+
+
+class TreePath(C.Structure):
+    """The accepted path of every tree (jamhip_tree_path); the arrays are device addresses of int32."""
+
+    _fields_ = [("ld_path", _I), ("path", _VP), ("accepted", _VP), ("next", _VP), ("lens", _VP), ("lens_out", _VP), ("slots", _VP),
+                ("move_from", _VP), ("move_to", _VP)]
+
+
 class Sampling(C.Structure):
     """Sampling parameters per row (jamhip_sampling), device addresses; None: temperature 1, no filter."""
 
@@ -42,6 +63,7 @@ class Sampling(C.Structure):
 
 
 _CACHE, _SPEC, _BATCH, _SAMPLING = (C.POINTER(t) for t in (KvCache, QkSpec, AttnBatch, Sampling))
+_PAGES, _TREE, _PATH = (C.POINTER(t) for t in (KvPages, Tree, TreePath))
 # (name, restype, argtypes) for every entry point of include/jamhip.h
 SIGNATURES = [
     ("jamhip_device_available", _I, []),
@@ -75,6 +97,11 @@ SIGNATURES = [
     ("jamhip_qkv_norm_rope_write", _I, [_VP, _SPEC, _CACHE, _VP, _I, _VP, _I, _VP, _I, _VP, _I, _VP, _VP, _I]),
     ("jamhip_kv_read", _I, [_VP, _CACHE, _VP, _I, _VP, _I, _VP, _I]),
     ("jamhip_attn_shared_prefix", _I, [_VP, _CACHE, _BATCH, _VP, _I, _I, C.c_float, _I, _VP, _VP, _I]),
+    ("jamhip_kv_resize", _I, [_VP, _PAGES]),
+    ("jamhip_tree_masks", _I, [_VP, _TREE, _VP, _I, _VP]),
+    ("jamhip_attn_tree", _I, [_VP, _CACHE, _BATCH, _VP, _I, _VP, _I, _I, C.c_float, _I, _VP, _VP, _I]),
+    ("jamhip_tree_accept", _I, [_VP, _TREE, _VP, _VP, _PATH]),
+    ("jamhip_kv_move", _I, [_VP, _CACHE, _I, _VP, _I, _VP, _VP, _I]),
     ("jamhip_sample", _I, [_VP, _VP, _I64, _I, _I, _SAMPLING, _VP, _VP]),
     ("jamhip_ctx_set_stream", _I, [_VP, _VP]),
     ("jamhip_ctx_stream", _VP, [_VP]),

@@ -48,6 +48,11 @@ UNITS = {   # source -> extra flags
     "attn_f16.hip": [],
     "attn_q8.hip": [],
     "attn_q4.hip": [],
+    "attn_tree_f16.hip": [],
+    "attn_tree_q8.hip": [],
+    "attn_tree_q4.hip": [],
+    "pages.hip": [],
+    "tree.hip": [],
     "sample.hip": [],
     "readfloor.hip": [],
     "jamhip.cpp": ["-x", "hip"],

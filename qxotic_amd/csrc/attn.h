@@ -5,6 +5,7 @@
 
 #include "kvcache.h"
 #include "launch.h"
+#include "treemask.h"
 
 namespace jamhip {
 
@@ -108,18 +109,31 @@ JAMHIP_DEV int64_t entry_row(const KvView& c, const SeqInfo& r, int at, int head
     return ((int64_t) ((uint32_t) p < (uint32_t) c.n_pages ? p : 0) * c.kv + head) * c.page.d + in;
 }
 
+// What query token `tok` of a sequence with these SeqInfo values sees (treemask.h).
+JAMHIP_DEV TreeMask tree_mask(const Attn& g, int tok) { return {g.masks + (int64_t) tok * g.mask_words, g.mask_words}; }
+JAMHIP_DEV TreeSpan tree_span(const Attn& g, int tok, const SeqInfo& s) {
+    return tree_span(tree_mask(g, tok), s.base, s.first, s.len - s.first, g.window);
+}
+
 constexpr int ATTN_ROW_FLOATS = 256 + 64;   // attn_row's shared memory: the query row, then a block's weights
 
 // One output row by one wave, every masked key left out entirely: 64 keys at a time, a key a lane for the scores, 4 elements
 // a lane for the values.
-template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, float* lds) {
+template <int TYPE, bool TREE = false> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, float* lds) {
     const int lane = threadIdx.x & 63, dim = g.cache.dim, kvh = g.grp.div(head);
     const int s = seq_of(g, t);
     if (s < 0) return;
     const SeqInfo r = seq_info(g, s);
     if (t - r.t0 >= r.nq) return;
     const int pos = r.base + r.first + (t - r.t0);
-    const int lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(r.base + r.len, pos + 1);
+    int lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(r.base + r.len, pos + 1);
+    TreeMask mask{};
+    TreeSpan span{};
+    if constexpr (TREE) {
+        mask = tree_mask(g, t);
+        span = tree_span(g, t, r);
+        lo = span_lo(span), hi = span_hi(span);
+    }
     float* qs = lds;
     float* ps = lds + 256;
     const float* q = g.q + t * g.ldq + (int64_t) head * dim;
@@ -129,8 +143,10 @@ template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, flo
     float4_t acc = {0, 0, 0, 0};
     for (int k0 = lo; k0 < hi; k0 += 64) {
         const int at = k0 + lane;
+        bool sees = at < hi;
+        if constexpr (TREE) sees = sees && span_sees(mask, span, at);
         float x = -__builtin_inff();
-        if (at < hi) {
+        if (sees) {
             const int64_t row = entry_row(g.cache, r, at, kvh);
             x = 0.0f;
             for (int d = 0; d < dim; d += 4) {
@@ -143,14 +159,16 @@ template <int TYPE> JAMHIP_DEV void attn_row(const Attn& g, int t, int head, flo
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
         const float now = fmaxf(m, top), ref = now == -__builtin_inff() ? 0.0f : now;
-        const float keep = expf(m - ref), p = at < hi ? expf(x - ref) : 0.0f;
+        const float keep = expf(m - ref), p = sees ? expf(x - ref) : 0.0f;
         l = l * keep + wave_sum(p);
         m = now;
         ps[lane] = p;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         acc *= keep;
+        const unsigned long long all = TREE ? __ballot(sees) : 0;
         if (4 * lane < dim)
             for (int j = 0; j < min(64, hi - k0); j++) {
+                if (TREE && !(all >> j & 1)) continue;
                 const int64_t row = entry_row(g.cache, r, k0 + j, kvh);
                 acc += kv_load4<TYPE>(g.cache.v, g.cache.scale_off, dim, row, 4 * lane) * ps[j];
             }

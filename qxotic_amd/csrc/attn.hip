@@ -9,13 +9,16 @@ namespace jamhip {
 hipError_t launch_attn_f16(const AttnArgs& a, hipStream_t st);
 hipError_t launch_attn_q8(const AttnArgs& a, hipStream_t st);
 hipError_t launch_attn_q4(const AttnArgs& a, hipStream_t st);
+hipError_t launch_attn_tree_f16(const AttnArgs& a, hipStream_t st);
+hipError_t launch_attn_tree_q8(const AttnArgs& a, hipStream_t st);
+hipError_t launch_attn_tree_q4(const AttnArgs& a, hipStream_t st);
 
 namespace {
 
 // 2048 rows of 128 in 33 parts, 35 MB: 9.9 us; with each part's load behind the one before 16.6.
 // One output row a wave: its parts (m_i, l_i, o_i) joined as Σ 2^(m_i - M) o_i / Σ 2^(m_i - M) l_i over the parts whose keys it
 // sees any of (no other part was written).
-template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, AttnPlan p) {
+template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, AttnPlan p) {
     __shared__ float redo[4][ATTN_ROW_FLOATS];
     const Attn& g = a.g;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -29,7 +32,12 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
     if (sq < 0) return;
     const SeqInfo s = small ? seq_info(g, lanes, sq) : seq_info(g, sq);
     if (t - s.t0 >= s.nq) return;
-    const int pos = s.base + s.first + (t - s.t0), lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(s.base + s.len, pos + 1);
+    const int pos = s.base + s.first + (t - s.t0);
+    int lo = g.window > 0 ? max(0, pos - g.window + 1) : 0, hi = min(s.base + s.len, pos + 1);
+    if constexpr (TREE) {   // parts between them whose keys it does not see hold a sum of zero
+        const TreeSpan span = tree_span(g, t, s);
+        lo = span_lo(span), hi = span_hi(span);
+    }
     constexpr int E = D > 128 ? 4 : D > 64 ? 2 : 1;   // elements a lane
     float m = -__builtin_inff(), l = 0.0f, o[E];
 #pragma unroll
@@ -89,17 +97,17 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
         const int d = lane * E + e;
         if (d < D) g.out[(int64_t) t * g.ldo + (int64_t) head * D + d] = o[e];
     }
-    if (__any(bad)) attn_row<TYPE>(g, t, head, redo[wave]);
+    if (__any(bad)) attn_row<TYPE, TREE>(g, t, head, redo[wave]);
 }
 
-template <int TYPE> hipError_t launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
+template <int TYPE, bool TREE> hipError_t launch_join(const AttnArgs& a, const AttnPlan& p, hipStream_t st) {
     return attn_runs(a, ((int64_t) a.g.n_tokens * a.g.heads + 3) / 4, [&](const AttnArgs& a, uint32_t blocks) {
         switch (a.g.cache.dim) {
-            case 64: attn_join_kernel<TYPE, 64><<<blocks, 256, 0, st>>>(a, p); break;
-            case 96: attn_join_kernel<TYPE, 96><<<blocks, 256, 0, st>>>(a, p); break;
-            case 128: attn_join_kernel<TYPE, 128><<<blocks, 256, 0, st>>>(a, p); break;
-            case 192: attn_join_kernel<TYPE, 192><<<blocks, 256, 0, st>>>(a, p); break;
-            case 256: attn_join_kernel<TYPE, 256><<<blocks, 256, 0, st>>>(a, p); break;
+            case 64: attn_join_kernel<TYPE, 64, TREE><<<blocks, 256, 0, st>>>(a, p); break;
+            case 96: attn_join_kernel<TYPE, 96, TREE><<<blocks, 256, 0, st>>>(a, p); break;
+            case 128: attn_join_kernel<TYPE, 128, TREE><<<blocks, 256, 0, st>>>(a, p); break;
+            case 192: attn_join_kernel<TYPE, 192, TREE><<<blocks, 256, 0, st>>>(a, p); break;
+            case 256: attn_join_kernel<TYPE, 256, TREE><<<blocks, 256, 0, st>>>(a, p); break;
             default: return hipErrorNotSupported;
         }
         return hipGetLastError();
@@ -125,14 +133,18 @@ hipError_t launch_attn(int type, const Attn& g, void* work, hipStream_t st) {
     a.g = g;
     a.acc = static_cast<float*>(work);
     a.ml = reinterpret_cast<float2*>(a.acc + (size_t) p.slots * g.n_tokens * g.heads * g.cache.dim);
+    const bool tree = g.masks != nullptr;
     for (int i = 0; i < p.n; i++) {
         a.part = p.part[i];
-        const hipError_t e = type == F16 ? launch_attn_f16(a, st) : type == Q8_0 ? launch_attn_q8(a, st)
-                           : type == Q4_0 ? launch_attn_q4(a, st) : hipErrorNotSupported;
+        const hipError_t e = type == F16    ? (tree ? launch_attn_tree_f16(a, st) : launch_attn_f16(a, st))
+                             : type == Q8_0 ? (tree ? launch_attn_tree_q8(a, st) : launch_attn_q8(a, st))
+                             : type == Q4_0 ? (tree ? launch_attn_tree_q4(a, st) : launch_attn_q4(a, st))
+                                            : hipErrorNotSupported;
         if (e != hipSuccess) return e;
     }
     if (p.slots == 0) return hipSuccess;
-    return type == F16 ? launch_join<F16>(a, p, st) : type == Q8_0 ? launch_join<Q8_0>(a, p, st) : launch_join<Q4_0>(a, p, st);
+    if (tree) return type == F16 ? launch_join<F16, true>(a, p, st) : type == Q8_0 ? launch_join<Q8_0, true>(a, p, st) : launch_join<Q4_0, true>(a, p, st);
+    return type == F16 ? launch_join<F16, false>(a, p, st) : type == Q8_0 ? launch_join<Q8_0, false>(a, p, st) : launch_join<Q4_0, false>(a, p, st);
 }
 
 }  // namespace jamhip

@@ -3,6 +3,6 @@
 
 namespace jamhip {
 
-hipError_t launch_attn_f16(const AttnArgs& a, hipStream_t st) { return launch_attn_part<F16>(a, st); }
+hipError_t launch_attn_f16(const AttnArgs& a, hipStream_t st) { return launch_attn_part<F16, false>(a, st); }
 
 }  // namespace jamhip

@@ -129,6 +129,7 @@ struct RowSet {
     SeqInfo s;         // the keys' tables (mode 1: the group's prefix alone)
     int r0, n_rows;    // its first row, rows of the set
     int t_first;       // the set's first token
+    int base_all;      // tokens of the sequence's prefix, in mode 2 too, whose keys are the own ones alone
     BatchLanes lanes;  // where the batch fits
 };
 
@@ -137,6 +138,7 @@ template <int ROWS> JAMHIP_DEV bool attn_row_set(const AttnArgs& a, int tile, Ro
     const Attn& g = a.g;
     const int lane = threadIdx.x & 63;
     w->s = SeqInfo{};
+    w->base_all = 0;
     const bool small = fits_lanes(g);
     if (small) w->lanes = batch_lanes(g);
     if (a.part.mode == 1 && small) {
@@ -181,6 +183,7 @@ template <int ROWS> JAMHIP_DEV bool attn_row_set(const AttnArgs& a, int tile, Ro
         w->t_first = w->s.t0;
         w->n_rows = w->s.nq * g.grp.d;
         w->r0 = (tile - q * per) * ROWS;
+        w->base_all = w->s.base;
         if (a.part.mode == 2) w->s.base = 0;   // positions among its own keys
     }
     return w->r0 < w->n_rows;
@@ -193,9 +196,11 @@ struct Column {
     int see_lo, see_n;     // key sees: (unsigned) (key - see_lo) <= see_n
     int lo, hi;            // the wave's first and last key that a row sees
     int all_lo, all_hi;    // between these every live row sees all
+    TreeSpan span;         // of a drafted tree's token: what it sees of the run
+    TreeMask mask;
 };
 
-JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowSet& w, int r, int kvh, int split) {
+template <bool TREE> JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowSet& w, int r, int kvh, int split) {
     const Attn& g = a.g;
     Column c;
     const int rr = min(r, w.n_rows - 1), total = w.s.base + w.s.len;
@@ -203,26 +208,43 @@ JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowSet& w, int r, int kvh
     c.head = kvh * g.grp.d + (rr - (c.tok - w.t_first) * g.grp.d);
     c.live = r < w.n_rows;
     int pos = w.s.base + w.s.first + (c.tok - w.s.t0);
+    int s_first = w.s.first, s_nq = w.s.len - w.s.first;
     if (a.part.mode == 1) {
         if (fits_lanes(g)) {   // the sequences of the wave's tokens, one after another
             const BatchLanes& b = w.lanes;
-            int at = 0, t0 = 0, nq = -1;   // at: SeqInfo::first
+            int at = 0, t0 = 0, nq = -1, whole = 0;   // at: SeqInfo::first
             const int t0_wave = wave_min(c.tok), t1_wave = wave_max(c.tok);
             unsigned long long on = __ballot(b.off < b.next && b.next > t0_wave && b.off <= t1_wave);
             for (; on; on &= on - 1) {
                 const int q = __ffsll(on) - 1, first = lane_int(b.off, q), end = lane_int(b.next, q);
-                if (c.tok >= first && c.tok < end) t0 = first, nq = min(end - first, g.max_q), at = lane_int(b.len, q) - (end - first);
+                if (c.tok >= first && c.tok < end)
+                    t0 = first, whole = end - first, nq = min(whole, g.max_q), at = lane_int(b.len, q) - whole;
             }
             c.live = c.live && c.tok - t0 < nq;
             pos = w.s.base + at + (c.tok - t0);
+            s_first = at, s_nq = whole;
         } else {
             const int q = seq_of(g, c.tok);
             const SeqInfo mine = seq_info(g, max(q, 0));
             c.live = c.live && q >= 0 && c.tok - mine.t0 < mine.nq;
             pos = mine.base + mine.first + (c.tok - mine.t0);
+            s_first = mine.first, s_nq = mine.len - mine.first;
         }
     }
     const int c0 = split * a.part.chunk;
+    if constexpr (TREE) {   // the context's keys, and the drafted ones' by their bits
+        c.mask = tree_mask(g, c.tok);
+        // the window counts the whole context's keys: in mode 2 positions are among the own ones
+        const int skip = a.part.mode == 2 ? w.base_all : 0;
+        c.span = span_cut(tree_span(c.mask, w.s.base + skip, s_first, s_nq, g.window), skip, c0, min(c0 + a.part.chunk, total));
+        const TreeHull h = span_hull(c.mask, c.span);
+        const bool some = c.live && h.lo <= h.hi, ctx = c.live && c.span.ctx_lo < c.span.ctx_hi;
+        c.see_lo = INT32_MAX, c.see_n = 0;
+        c.lo = wave_min(some ? h.lo : INT32_MAX), c.hi = wave_max(some ? h.hi : -1);
+        c.all_lo = wave_max(c.live ? (ctx ? c.span.ctx_lo : INT32_MAX) : -1);
+        c.all_hi = wave_min(c.live ? (ctx ? c.span.ctx_hi - 1 : -1) : INT32_MAX);
+        return c;
+    }
     const int k_lo = max(c0, g.window > 0 ? pos - g.window + 1 : 0), k_hi = min(min(total, c0 + a.part.chunk) - 1, pos);   // first and last
     const bool some = c.live && k_lo <= k_hi;
     c.see_lo = some ? k_lo : INT32_MAX, c.see_n = some ? k_hi - k_lo : 0;
@@ -232,9 +254,16 @@ JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowSet& w, int r, int kvh
 }
 
 // ---- the softmax's step: a tile's scores sc (of ST products' accumulators) become weights; o and l follow the maximum
-template <typename M, int ST, int DT, int NC, typename ACC>
+template <typename M, int ST, int DT, int NC, bool TREE, typename ACC>
 JAMHIP_DEV void attn_weights(ACC (&sc)[ST], ACC (&o)[DT], float& m, float& l, float f, const Column& c, int kw, int part) {
-    if (kw < c.all_lo || kw + ST * NC - 1 > c.all_hi) {
+    if (TREE && (kw < c.all_lo || kw + ST * NC - 1 > c.all_hi)) {
+        const uint64_t sees = span_tile(c.mask, c.span, kw) >> (4 * part);   // M::row(k, part) = M::row(k, 0) + 4 · part
+#pragma unroll
+        for (int i = 0; i < ST; i++)
+#pragma unroll
+            for (int k = 0; k < M::N; k++)
+                if (!(sees >> (i * NC + M::row(k, 0)) & 1)) sc[i][k] = -__builtin_inff();
+    } else if (!TREE && (kw < c.all_lo || kw + ST * NC - 1 > c.all_hi)) {
 #pragma unroll
         for (int i = 0; i < ST; i++)
 #pragma unroll

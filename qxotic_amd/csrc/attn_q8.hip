@@ -3,6 +3,6 @@
 
 namespace jamhip {
 
-hipError_t launch_attn_q8(const AttnArgs& a, hipStream_t st) { return launch_attn_part<Q8_0>(a, st); }
+hipError_t launch_attn_q8(const AttnArgs& a, hipStream_t st) { return launch_attn_part<Q8_0, false>(a, st); }
 
 }  // namespace jamhip

@@ -26,7 +26,7 @@ template <int TYPE, int D> struct Tile {
     static constexpr int STEPS = D / M::DEPTH, ST = KEYS / NC, DT = D / NC;
 };
 
-template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
+template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256, D <= 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
     using T = Tile<TYPE, D>;
     using M = typename T::M;
     using acc_t = typename M::acc_t;
@@ -46,7 +46,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
     const int tile = rows_last ? b / a.part.splits : b % a.part.tiles, split = rows_last ? b % a.part.splits : b / a.part.tiles;
     RowSet w;
     if (!attn_row_set<T::ROWS>(a, tile, &w)) return;
-    const Column c = attn_column(a, w, w.r0 + wave * NC + col, kvh, split);
+    const Column c = attn_column<TREE>(a, w, w.r0 + wave * NC + col, kvh, split);
     if (lane == 0) range[0][wave] = c.lo, range[1][wave] = c.hi;
     half8_t qh[T::STEPS], ql[T::STEPS];
     const float f = load_query<NC>(g.q + (int64_t) c.tok * g.ldq + (int64_t) c.head * D, g.scale, qh, ql,
@@ -119,7 +119,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
 #pragma unroll
                 for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], ql[st], sc[i]);
             }
-            attn_weights<M, T::ST, T::DT, NC>(sc, o, m, l, f, c, k0, part);
+            attn_weights<M, T::ST, T::DT, NC, TREE>(sc, o, m, l, f, c, k0, part);
 #pragma unroll
             for (int u = 0; u < KEYS / M::DEPTH; u++) {
                 half8_t ph, pl;
@@ -132,7 +132,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256, D <= 128 ? 2 :
     l = column_sum<NC>(l);
     for (unsigned long long again = attn_emit<D, NC, T::DT, 1, M>(a, c, o, m, l, split, 0); again; again &= again - 1) {
         const int k = __ffsll(again) - 1;
-        attn_row<TYPE>(g, __builtin_amdgcn_readlane(c.tok, k), __builtin_amdgcn_readlane(c.head, k), redo[wave]);
+        attn_row<TYPE, TREE>(g, __builtin_amdgcn_readlane(c.tok, k), __builtin_amdgcn_readlane(c.head, k), redo[wave]);
     }
 }
 

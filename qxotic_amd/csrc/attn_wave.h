@@ -116,7 +116,7 @@ template <int TYPE, int D, int NC> struct Wave {
 // waves a SIMD that the registers are to leave room for
 constexpr int wave_occupancy(int dim, int nc) { return dim >= 192 ? 1 : nc == 16 && dim == 64 ? 3 : 2; }
 
-template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_occupancy(D, NC))) attn_wave_kernel(AttnArgs a) {
+template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(256, (wave_occupancy(D, NC))) attn_wave_kernel(AttnArgs a) {
     using T = Wave<TYPE, D, NC>;
     using M = typename T::M;
     using acc_t = typename M::acc_t;
@@ -134,7 +134,7 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
     const int tile = rows_last ? b / a.part.splits : b % a.part.tiles, split = rows_last ? b % a.part.splits : b / a.part.tiles;
     RowSet w;
     if (!attn_row_set<T::ROWS>(a, tile, &w)) return;
-    const Column c = attn_column(a, w, w.r0 + col, kvh, split);
+    const Column c = attn_column<TREE>(a, w, w.r0 + col, kvh, split);
     const int lo = c.lo, hi = c.hi + 1;   // the same in every wave
 
     half8_t qh[T::STEPS], ql[T::STEPS];
@@ -204,7 +204,7 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
             fetch_k(rw[buf]);
             if (lane < T::KEYS && k0 + 2 * step < hi) after = row_of(k0 + 2 * step + lane);
         }
-        attn_weights<M, T::ST, T::DT, NC>(sc, o, m, l, f, c, k0, part);
+        attn_weights<M, T::ST, T::DT, NC, TREE>(sc, o, m, l, f, c, k0, part);
         sync();   // the values are in shared memory
 #pragma unroll
         for (int u = 0; u < T::KEYS / M::DEPTH; u++) {
@@ -255,7 +255,7 @@ template <int TYPE, int D, int NC> __global__ void __launch_bounds__(256, (wave_
     __syncthreads();   // a row that one wave finds not finite is whole before it is written again
     for (; again; again &= again - 1) {
         const int k = __ffsll(again) - 1;
-        attn_row<TYPE>(g, __builtin_amdgcn_readlane(c.tok, k), __builtin_amdgcn_readlane(c.head, k), redo[wave]);
+        attn_row<TYPE, TREE>(g, __builtin_amdgcn_readlane(c.tok, k), __builtin_amdgcn_readlane(c.head, k), redo[wave]);
     }
 }
 

@@ -16,6 +16,7 @@
 #include "common.h"
 #include "gguf.h"
 #include "launch.h"
+#include "treeargs.h"
 
 using namespace jamhip;
 
@@ -1264,8 +1265,9 @@ jamhip_status kv_read_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const void
     return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "kv_read launch");
 }
 
+// masks (words of them a row): the query tokens are drafted trees; null: each sees those before it
 jamhip_status attn_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const jamhip_attn_batch* b, const void* q, int ldq, int heads,
-                        float scale, int window, const void* sinks, void* out, int ldo) {
+                        float scale, int window, const void* sinks, void* out, int ldo, const void* masks = nullptr, int words = 0) {
     if (!ctx) return JAMHIP_EINVAL;
     const jamhip_status st = kv_valid(ctx, "attn", c, true);
     if (st != JAMHIP_OK) return st;
@@ -1300,10 +1302,104 @@ jamhip_status attn_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const jamhip_
     g.prefix_pages = (const int*) b->prefix_pages;
     g.ld_seq_pages = b->ld_seq_pages, g.ld_prefix_pages = b->ld_prefix_pages;
     g.grp = FastDiv(heads / c->kv_heads);
+    g.masks = (const uint64_t*) masks, g.mask_words = words;
     hipError_t e = ctx->attn.ensure(attn_workspace(g));
     if (e != hipSuccess) return hip_fail(ctx, e, "attn workspace");
     e = launch_attn(c->type, g, ctx->attn.p, ctx->stream);
     return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "attn launch");
+}
+
+jamhip_status refused(jamhip_ctx* ctx, const Refusal& r) { return fail(ctx, r.status, r.why); }
+
+jamhip_status attn_tree_impl(jamhip_ctx* ctx, const jamhip_kv_cache* c, const jamhip_attn_batch* b, const void* masks, int words, const void* q,
+                             int ldq, int heads, float scale, int window, const void* sinks, void* out, int ldo) {
+    if (!ctx) return JAMHIP_EINVAL;
+    if (!b) return fail(ctx, JAMHIP_EINVAL, "attn: null operand");
+    const Refusal r = refuse_masks(masks, words, b->max_q);
+    if (r.status != JAMHIP_OK) return refused(ctx, r);
+    return attn_impl(ctx, c, b, q, ldq, heads, scale, window, sinks, out, ldo, masks, words);
+}
+
+jamhip_status kv_resize_impl(jamhip_ctx* ctx, const jamhip_kv_pages* p) {
+    if (!ctx) return JAMHIP_EINVAL;
+    const Refusal r = refuse_pages(p);
+    if (r.status != JAMHIP_OK) return refused(ctx, r);
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    Pages g{};
+    g.n_seqs = p->n_seqs, g.n_tokens = p->n_tokens, g.n_pages = p->n_pages, g.free_cap = p->free_cap, g.ld = p->ld_seq_pages;
+    g.page = FastDiv(p->page_tokens);
+    g.lens = (const int*) p->lens, g.targets = (const int*) p->targets, g.base = (const int*) p->base, g.held = (const int*) p->held;
+    g.n_free = (const int*) p->n_free, g.free_pages = (int*) p->free_pages, g.seq_pages = (int*) p->seq_pages;
+    g.lens_out = (int*) p->lens_out, g.held_out = (int*) p->held_out, g.n_free_out = (int*) p->n_free_out, g.status = (int*) p->status;
+    g.q_offsets = (int*) p->q_offsets, g.pos = (int*) p->pos, g.slots = (int*) p->slots;
+    const hipError_t e = launch_kv_resize(g, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "kv_resize launch");
+}
+
+Trees trees_of(const jamhip_tree* t) {
+    Trees g{};
+    g.n_tokens = t->n_tokens, g.n_seqs = t->n_seqs, g.max_q = t->max_q;
+    g.q_offsets = (const int*) t->q_offsets, g.parents = (const int*) t->parents;
+    return g;
+}
+
+jamhip_status tree_masks_impl(jamhip_ctx* ctx, const jamhip_tree* t, void* masks, int words, void* pos) {
+    if (!ctx) return JAMHIP_EINVAL;
+    Refusal r = refuse_tree(t);
+    if (r.status == JAMHIP_OK) r = refuse_masks(masks, words, t->max_q);
+    if (r.status != JAMHIP_OK) return refused(ctx, r);
+    if (t->n_tokens == 0 || t->n_seqs == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    const hipError_t e = launch_tree_masks(trees_of(t), (uint64_t*) masks, words, (int*) pos, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "tree_masks launch");
+}
+
+jamhip_status tree_accept_impl(jamhip_ctx* ctx, const jamhip_tree* t, const void* tokens, const void* picked, const jamhip_tree_path* p) {
+    if (!ctx) return JAMHIP_EINVAL;
+    Refusal r = refuse_tree(t);
+    if (r.status == JAMHIP_OK && t->n_seqs > 0 && !t->q_offsets) r = {JAMHIP_EINVAL, "tree: null array"};
+    if (r.status == JAMHIP_OK) r = refuse_path(t, tokens, picked, p);
+    if (r.status != JAMHIP_OK) return refused(ctx, r);
+    if (t->n_seqs == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    TreeWalk w{};
+    w.tokens = (const int*) tokens, w.picked = (const int*) picked, w.lens = (const int*) p->lens, w.slots = (const int*) p->slots;
+    w.path = (int*) p->path, w.accepted = (int*) p->accepted, w.next = (int*) p->next, w.lens_out = (int*) p->lens_out;
+    w.from = (int*) p->move_from, w.to = (int*) p->move_to, w.ld_path = p->ld_path;
+    const hipError_t e = launch_tree_accept(trees_of(t), w, ctx->stream);
+    return e == hipSuccess ? JAMHIP_OK : hip_fail(ctx, e, "tree_accept launch");
+}
+
+jamhip_status kv_move_impl(jamhip_ctx* ctx, const jamhip_kv_cache* caches, int n_caches, const void* offsets, int n_groups, const void* from,
+                           const void* to, int n) {
+    if (!ctx) return JAMHIP_EINVAL;
+    const Refusal r = refuse_move(caches, n_caches, offsets, n_groups, from, to, n);
+    if (r.status != JAMHIP_OK) return refused(ctx, r);
+    for (int i = 0; i < n_caches; i++) {
+        const jamhip_status st = kv_valid(ctx, "kv_move", caches + i, true);
+        if (st != JAMHIP_OK) return st;
+    }
+    if (n_caches == 0 || n_groups == 0 || n == 0) return JAMHIP_OK;
+    Busy guard(ctx);
+    if (!guard.ok) return fail(ctx, JAMHIP_EBUSY, "context busy");
+    (void) hipSetDevice(ctx->device);
+    Move g{};
+    g.cache = kv_view(caches);
+    g.n = n, g.groups = n_groups;
+    g.offsets = (const int*) offsets, g.from = (const int*) from, g.to = (const int*) to;
+    for (int i = 0; i < n_caches; i += MOVE_CACHES) {
+        g.n_caches = n_caches - i < MOVE_CACHES ? n_caches - i : MOVE_CACHES;
+        for (int j = 0; j < g.n_caches; j++) g.k[j] = static_cast<uint8_t*>(caches[i + j].k), g.v[j] = static_cast<uint8_t*>(caches[i + j].v);
+        const hipError_t e = launch_kv_move(caches->type, g, ctx->stream);
+        if (e != hipSuccess) return hip_fail(ctx, e, "kv_move launch");
+    }
+    return JAMHIP_OK;
 }
 
 jamhip_status sample_impl(jamhip_ctx* ctx, const void* logits, int64_t ld, int rows, int vocab, const jamhip_sampling* p,
@@ -1653,6 +1749,32 @@ jamhip_status jamhip_attn_shared_prefix(jamhip_ctx* ctx, const jamhip_kv_cache* 
     return on_ctx(ctx, [&](jamhip_ctx* x) {
         return attn_impl(x, cache, batch, q_dev, ldq, q_heads, scale, window, sinks_dev, out_dev, ldo);
     });
+}
+
+jamhip_status jamhip_kv_resize(jamhip_ctx* ctx, const jamhip_kv_pages* pages) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) { return kv_resize_impl(x, pages); });
+}
+
+jamhip_status jamhip_tree_masks(jamhip_ctx* ctx, const jamhip_tree* tree, void* masks_dev, int mask_words, void* pos_dev) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) { return tree_masks_impl(x, tree, masks_dev, mask_words, pos_dev); });
+}
+
+jamhip_status jamhip_attn_tree(jamhip_ctx* ctx, const jamhip_kv_cache* cache, const jamhip_attn_batch* batch, const void* masks_dev,
+                               int mask_words, const void* q_dev, int ldq, int q_heads, float scale, int window, const void* sinks_dev,
+                               void* out_dev, int ldo) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) {
+        return attn_tree_impl(x, cache, batch, masks_dev, mask_words, q_dev, ldq, q_heads, scale, window, sinks_dev, out_dev, ldo);
+    });
+}
+
+jamhip_status jamhip_tree_accept(jamhip_ctx* ctx, const jamhip_tree* tree, const void* tokens_dev, const void* picked_dev,
+                                 const jamhip_tree_path* path) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) { return tree_accept_impl(x, tree, tokens_dev, picked_dev, path); });
+}
+
+jamhip_status jamhip_kv_move(jamhip_ctx* ctx, const jamhip_kv_cache* caches, int n_caches, const void* offsets_dev, int n_groups,
+                             const void* from_dev, const void* to_dev, int n) {
+    return on_ctx(ctx, [&](jamhip_ctx* x) { return kv_move_impl(x, caches, n_caches, offsets_dev, n_groups, from_dev, to_dev, n); });
 }
 
 jamhip_status jamhip_sample(jamhip_ctx* ctx, const void* logits_dev, int64_t ld, int rows, int vocab,

@@ -313,8 +313,68 @@ struct Attn {
     const int* prefix_pages;
     int ld_seq_pages, ld_prefix_pages;
     FastDiv grp;   // query heads per key head
+    // drafted trees: bit j of row t says that query token t sees its sequence's query token j; null: those before it and itself
+    const uint64_t* masks;   // [n_tokens][mask_words]
+    int mask_words;
 };
 size_t attn_workspace(const Attn& g);   // bytes of `work`
 hipError_t launch_attn(int type, const Attn& g, void* work, hipStream_t st);
+
+// Page tables and slots from the sequences' lengths (pages.hip); the *_out arrays may be those that they follow from.
+struct Pages {
+    int n_seqs, n_tokens, n_pages, free_cap, ld;
+    FastDiv page;   // page.d = tokens per page
+    const int* lens;
+    const int* targets;
+    const int* base;
+    const int* held;
+    const int* n_free;
+    int* free_pages;
+    int* seq_pages;
+    int* lens_out;
+    int* held_out;
+    int* n_free_out;
+    int* status;
+    int* q_offsets;
+    int* pos;
+    int* slots;
+};
+hipError_t launch_kv_resize(const Pages& g, hipStream_t st);
+
+// Entries of slots copied to others in up to MOVE_CACHES caches of one shape at once (pages.hip).
+constexpr int MOVE_CACHES = 128;
+struct Move {
+    KvView cache;   // the shape; k and v of each cache below
+    uint8_t* k[MOVE_CACHES];
+    uint8_t* v[MOVE_CACHES];
+    int n_caches, n, groups;
+    const int* offsets;
+    const int* from;
+    const int* to;
+};
+hipError_t launch_kv_move(int type, const Move& g, hipStream_t st);
+
+// Drafted trees (tree.hip): a sequence's tokens, each one's parent among them.
+struct Trees {
+    int n_tokens, n_seqs, max_q;
+    const int* q_offsets;
+    const int* parents;
+};
+hipError_t launch_tree_masks(const Trees& g, uint64_t* masks, int words, int* pos, hipStream_t st);
+
+struct TreeWalk {
+    const int* tokens;
+    const int* picked;
+    const int* lens;
+    const int* slots;
+    int* path;
+    int* accepted;
+    int* next;
+    int* lens_out;
+    int* from;
+    int* to;
+    int ld_path;
+};
+hipError_t launch_tree_accept(const Trees& g, const TreeWalk& w, hipStream_t st);
 
 }  // namespace jamhip

@@ -1,0 +1,255 @@
+// Pages of the cache handed out and taken back by the sequences' lengths, their slots, and entries moved between slots.
+//
+//   need_s  = ceil(target_s / page)                       back_s = max(0, held_s - need_s)     take_s = max(0, need_s - held_s)
+//   pages given back go on the list of free ones from the last sequence to the first, each one's last page first; then the sequences take
+//   theirs off its end in their order, so that giving back at once what was taken restores the list
+//   q_offsets = the sums of max(0, target - len) before, slot(p) = seq_pages[p / page] · page + p % page
+//
+// Small integers in a chain: what counts is the number of launches and of rounds of dependent loads. Lists and counts are device data:
+// whatever they hold, no index leaves the arrays.
+#include "launch.h"
+
+namespace jamhip {
+
+namespace {
+
+constexpr int T = 1024;   // threads, and sequences at once, of the workgroup that hands out pages
+
+// exclusive sums of v over the workgroup's threads; *total gets the whole. `lds`: T / 64 + 1 entries, free again after the next barrier
+JAMHIP_DEV int64_t block_scan(int64_t v, int64_t* lds, int64_t* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = x;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+    for (int i = 0; i < T / 64; i++) {
+        before += i < wave ? lds[i] : 0;
+        all += lds[i];
+    }
+    *total = all;
+    return before + x - v;
+}
+
+struct Want {
+    int len, target, held, need;
+    int64_t fresh;   // new tokens
+};
+JAMHIP_DEV Want want_of(const Pages& g, int s) {
+    Want w{};
+    if (s < g.n_seqs) {
+        w.len = max(g.lens[s], 0);
+        w.target = max(g.targets[s], 0);
+        w.held = min(max(g.held[s], 0), g.ld);
+        w.need = g.page.div(w.target) + (g.page.div(w.target) * g.page.d < w.target);
+        w.fresh = max(0, w.target - w.len);
+    }
+    return w;
+}
+
+// the last i in [0, n) with a[i] <= v, a rising from a[0] <= v
+JAMHIP_DEV int find_last(const int64_t* a, int n, int64_t v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= v) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(T) kv_resize_kernel(Pages g) {
+    __shared__ int64_t scan[T / 64 + 1];
+    __shared__ int64_t start[T];   // a chunk's sequences: pages given back or taken before each
+    __shared__ int first[T];       // and the first page's place in its row
+    __shared__ int stop;           // the first sequence of a chunk that does not fit
+    const int tid = threadIdx.x;
+    const int64_t free0 = min(max(g.n_free[0], 0), g.free_cap);
+    int64_t total = 0, sum;
+    for (int s0 = 0; s0 < g.n_seqs; s0 += T) {
+        const Want w = want_of(g, s0 + tid);
+        (void) block_scan(max(0, w.held - w.need), scan, &sum);
+        total += sum;
+    }
+    if (total > 0) {
+        int64_t done = 0;
+        for (int s0 = 0; s0 < g.n_seqs; s0 += T) {
+            const Want w = want_of(g, s0 + tid);
+            const int64_t at = block_scan(max(0, w.held - w.need), scan, &sum);
+            start[tid] = at, first[tid] = w.need;
+            __syncthreads();
+            for (int64_t k = tid; k < sum; k += T) {
+                const int i = find_last(start, T, k);
+                // k counts from the row's first page that goes back; on the list it stands that far from the end
+                const int64_t place = free0 + total - 1 - (done + k);
+                if (place < g.free_cap) g.free_pages[place] = g.seq_pages[(int64_t) (s0 + i) * g.ld + first[i] + (k - start[i])];
+            }
+            __syncthreads();
+            done += sum;
+        }
+    }
+    __threadfence_block();
+    __syncthreads();
+    const int64_t have = min(free0 + total, (int64_t) g.free_cap);
+    int64_t taken = 0, rows = 0, given = 0;   // pages asked for, tokens, pages handed out by the sequences before
+    bool full = false;
+    for (int s0 = 0; s0 < g.n_seqs; s0 += T) {
+        const int s = s0 + tid;
+        const Want w = want_of(g, s);
+        const int64_t take = max(0, w.need - w.held);
+        int64_t asked, all_rows;
+        const int64_t at = block_scan(take, scan, &asked);
+        const int64_t row = block_scan(w.fresh, scan, &all_rows);
+        const bool grows = take > 0 || w.fresh > 0;
+        if (tid == 0) stop = full ? 0 : T;
+        __syncthreads();
+        if (!full && grows && (taken + at + take > have || rows + row + w.fresh > g.n_tokens || w.need > g.ld)) atomicMin(&stop, tid);
+        __syncthreads();
+        const bool refused = grows && tid >= stop;
+        start[tid] = at, first[tid] = w.held;
+        if (s < g.n_seqs) {
+            g.lens_out[s] = refused ? w.len : w.target;
+            g.held_out[s] = refused ? w.held : w.need;
+            g.status[s] = refused;
+            g.q_offsets[s] = (int) min(rows + row, (int64_t) g.n_tokens);
+        }
+        __syncthreads();
+        const int64_t served = stop < T ? (full ? 0 : start[stop]) : asked;
+        for (int64_t k = tid; k < served; k += T) {
+            const int i = find_last(start, T, k);
+            g.seq_pages[(int64_t) (s0 + i) * g.ld + first[i] + (k - start[i])] = g.free_pages[have - 1 - (taken + k)];
+        }
+        full = full || stop < T;
+        taken += asked, rows += all_rows, given += served;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        g.q_offsets[g.n_seqs] = (int) min(rows, (int64_t) g.n_tokens);
+        g.n_free_out[0] = (int) (have - given);
+    }
+}
+
+constexpr int FILL = 256;
+
+// One token a thread: its sequence, position and slot.
+__global__ void __launch_bounds__(FILL) kv_slots_kernel(Pages g) {
+    const int t = blockIdx.x * FILL + threadIdx.x;
+    if (t >= g.n_tokens) return;
+    int lo = 0, hi = g.n_seqs + 1;   // the last offset not above t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (g.q_offsets[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    int pos = 0, slot = -1;
+    if (lo < g.n_seqs) {
+        const int o0 = g.q_offsets[lo], n = g.q_offsets[lo + 1] - o0;
+        const bool refused = g.status[lo] != 0;
+        const int p = g.lens_out[lo] - (refused ? 0 : n) + (t - o0);   // the length before and on
+        pos = p + (g.base != nullptr ? g.base[lo] : 0);
+        if (!refused && p >= 0) {
+            const int c = g.page.div(p);
+            const int page = c < g.ld ? g.seq_pages[(int64_t) lo * g.ld + c] : -1;
+            if ((uint32_t) page < (uint32_t) g.n_pages) slot = page * g.page.d + (p - c * g.page.d);
+        }
+    }
+    g.pos[t] = pos;
+    g.slots[t] = slot;
+}
+
+// ---- entries moved
+// A workgroup moves one group's entries in one cache: a thread holds the same piece of every entry, so that the entries of a group go in their
+// order without a barrier between them.
+constexpr int BATCH = 4;
+
+template <typename U> JAMHIP_DEV void move_pieces(uint8_t* buf, int64_t plane, int pieces, int per_head, const KvView& c, const int* pf,
+                                                  const int* at_f, const int* pt, const int* at_t, int n) {
+    for (int u = threadIdx.x; u < pieces; u += blockDim.x) {
+        const int head = u / per_head, at = u - head * per_head;
+        U v[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (i < n) v[i] = reinterpret_cast<const U*>(buf + plane)[(((int64_t) pf[i] * c.kv + head) * c.page.d + at_f[i]) * per_head + at];
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+            if (i < n) reinterpret_cast<U*>(buf + plane)[(((int64_t) pt[i] * c.kv + head) * c.page.d + at_t[i]) * per_head + at] = v[i];
+    }
+}
+
+template <int TYPE> __global__ void __launch_bounds__(256) kv_move_kernel(Move g, int block0) {
+    const int b = block0 + blockIdx.x, cache = b % g.n_caches, grp = b / g.n_caches;
+    const KvView& c = g.cache;
+    const int e0 = min(max(g.offsets[grp], 0), g.n), e1 = min(max(g.offsets[grp + 1], e0), g.n);
+    const int lane = threadIdx.x & 63;
+    for (int s0 = e0; s0 < e1; s0 += 64) {
+        const int e = s0 + lane;
+        int f = -1, t = -1;
+        if (e < e1) f = g.from[e], t = g.to[e];
+        const int64_t slots = c.slots();
+        unsigned long long on = __ballot(f >= 0 && t >= 0 && f < slots && t < slots && f != t);
+        while (on) {
+            // up to BATCH entries whose sources no earlier one of them writes
+            int pf[BATCH], at_f[BATCH], pt[BATCH], at_t[BATCH], to[BATCH], n = 0;
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) {
+                pf[i] = at_f[i] = pt[i] = at_t[i] = 0, to[i] = -1;
+                if (on && n == i) {
+                    const int l = __ffsll(on) - 1;
+                    const int ff = __builtin_amdgcn_readlane(f, l), tt = __builtin_amdgcn_readlane(t, l);
+                    bool clash = false;
+#pragma unroll
+                    for (int j = 0; j < i; j++) clash |= to[j] == ff;
+                    if (!clash) {
+                        pf[i] = c.page.div(ff), at_f[i] = ff - pf[i] * c.page.d;
+                        pt[i] = c.page.div(tt), at_t[i] = tt - pt[i] * c.page.d;
+                        to[i] = tt;
+                        n = i + 1;
+                        on &= on - 1;
+                    }
+                }
+            }
+            const int row = kv_row_bytes(TYPE, c.dim) / 16, sc = kv_scales(TYPE, c.dim);
+            move_pieces<uint4_t>(g.k[cache], 0, c.kv * row, row, c, pf, at_f, pt, at_t, n);
+            move_pieces<uint4_t>(g.v[cache], 0, c.kv * row, row, c, pf, at_f, pt, at_t, n);
+            if (TYPE != F16) {
+                move_pieces<uint16_t>(g.k[cache], c.scale_off, c.kv * sc, sc, c, pf, at_f, pt, at_t, n);
+                move_pieces<uint16_t>(g.v[cache], c.scale_off, c.kv * sc, sc, c, pf, at_f, pt, at_t, n);
+            }
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_kv_resize(const Pages& g, hipStream_t st) {
+    kv_resize_kernel<<<1, T, 0, st>>>(g);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || g.n_tokens == 0) return e;
+    kv_slots_kernel<<<(g.n_tokens + FILL - 1) / FILL, FILL, 0, st>>>(g);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_move(int type, const Move& g, hipStream_t st) {
+    const int64_t blocks = (int64_t) g.groups * g.n_caches;
+    constexpr int64_t RUN = 1 << 23;   // HIP takes fewer than 2^32 threads a launch
+    if (blocks > INT32_MAX) return hipErrorNotSupported;
+    for (int64_t b = 0; b < blocks; b += RUN) {
+        const uint32_t n = (uint32_t) (blocks - b < RUN ? blocks - b : RUN);
+        switch (type) {
+            case F16: kv_move_kernel<F16><<<n, 256, 0, st>>>(g, (int) b); break;
+            case Q8_0: kv_move_kernel<Q8_0><<<n, 256, 0, st>>>(g, (int) b); break;
+            case Q4_0: kv_move_kernel<Q4_0><<<n, 256, 0, st>>>(g, (int) b); break;
+            default: return hipErrorNotSupported;
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace jamhip

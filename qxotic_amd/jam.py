@@ -26,7 +26,7 @@ from typing import Any
 import numpy as np
 
 from . import ggml
-from ._lib import AttnBatch, KvCache, QkSpec, Sampling, lib, on_exit, register_for_teardown
+from ._lib import AttnBatch, KvCache, KvPages, QkSpec, Sampling, Tree, TreePath, lib, on_exit, register_for_teardown
 
 
 class JAM:
@@ -337,6 +337,28 @@ class HipJAM:
         """Attention of a ragged batch over the cache, prefixes shared by groups of sequences (jamhip_attn_shared_prefix)."""
         return lib().jamhip_attn_shared_prefix(self.ctx, cache, batch, q_dev, ldq, q_heads, scale, window, sinks_dev, out_dev, ldo)
 
+    def kv_resize(self, pages: KvPages) -> int:
+        """Pages handed out and taken back by the sequences' lengths, and the new tokens' slots (jamhip_kv_resize)."""
+        return lib().jamhip_kv_resize(self.ctx, pages)
+
+    def tree_masks(self, tree: Tree, masks_dev: int, mask_words: int, pos_dev: int | None = None) -> int:
+        """What each drafted token sees of its tree, and its position (jamhip_tree_masks)."""
+        return lib().jamhip_tree_masks(self.ctx, tree, masks_dev, mask_words, pos_dev)
+
+    def attn_tree(self, cache: KvCache, batch: AttnBatch, masks_dev: int, mask_words: int, q_dev: int, ldq: int, q_heads: int, scale: float,
+                  out_dev: int, ldo: int, window: int = 0, sinks_dev: int | None = None) -> int:
+        """attn_shared_prefix with drafted trees as the query tokens (jamhip_attn_tree)."""
+        return lib().jamhip_attn_tree(self.ctx, cache, batch, masks_dev, mask_words, q_dev, ldq, q_heads, scale, window, sinks_dev, out_dev,
+                                      ldo)
+
+    def tree_accept(self, tree: Tree, tokens_dev: int, picked_dev: int, path: TreePath) -> int:
+        """The drafted tokens that the model's picks agree with, a path of each tree (jamhip_tree_accept)."""
+        return lib().jamhip_tree_accept(self.ctx, tree, tokens_dev, picked_dev, path)
+
+    def kv_move(self, caches, n_caches: int, offsets_dev: int, n_groups: int, from_dev: int, to_dev: int, n: int) -> int:
+        """Entries moved between slots in each of `caches`, a KvCache or an array of them (jamhip_kv_move)."""
+        return lib().jamhip_kv_move(self.ctx, caches, n_caches, offsets_dev, n_groups, from_dev, to_dev, n)
+
     def sample(self, logits_dev: int, ld: int, rows: int, vocab: int, params: Sampling, token_dev: int,
                logprob_dev: int | None = None) -> int:
         """The next token of each row of logits from given random numbers (jamhip_sample)."""
@@ -448,4 +470,4 @@ def addr(x) -> int:
 
 
 __all__ = ["JAM", "HipJAM", "Provider", "providers", "register", "Segment", "IllegalArgumentError",
-           "IndexOutOfBoundsError", "addr", "C", "AttnBatch", "KvCache", "QkSpec", "Sampling"]
+           "IndexOutOfBoundsError", "addr", "C", "AttnBatch", "KvCache", "KvPages", "QkSpec", "Sampling", "Tree", "TreePath"]

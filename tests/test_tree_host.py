@@ -1,0 +1,141 @@
+"""CPU: which keys a drafted token sees (csrc/treemask.h) against the list of them, what the calls around drafted trees refuse
+(csrc/treeargs.h), both compiled without HIP, and the layout of the structs of the binding."""
+import ctypes
+import random
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+from oracle import tree as T
+
+ROOT = Path(__file__).resolve().parent.parent
+SHIM = """
+#include "treemask.h"
+#include "treeargs.h"
+using namespace jamhip;
+// o: see_lo, see_hi, hull lo, hull hi; sees[n], tiles[n]: 64 bits from key i on
+extern "C" void q_span(const uint64_t* row, int words, int base, int first, int nq, int window, int skip, int c0, int c1, int n, int* o, int* sees, uint64_t* tiles) {
+    const TreeMask m{row, words};
+    const TreeSpan s = span_cut(tree_span(m, base, first, nq, window), skip, c0, c1);
+    const TreeHull h = span_hull(m, s);
+    o[0] = span_lo(s), o[1] = span_hi(s), o[2] = h.lo, o[3] = h.hi;
+    for (int i = 0; i < n; i++) sees[i] = span_sees(m, s, i), tiles[i] = span_tile(m, s, i);
+}
+extern "C" int q_pages(const jamhip_kv_pages* p) { return refuse_pages(p).status; }
+extern "C" int q_tree(const jamhip_tree* p) { return refuse_tree(p).status; }
+extern "C" int q_masks(const void* m, int words, int max_q) { return refuse_masks(m, words, max_q).status; }
+extern "C" int q_path(const jamhip_tree* t, const void* a, const void* b, const jamhip_tree_path* p) { return refuse_path(t, a, b, p).status; }
+extern "C" int q_move(const jamhip_kv_cache* c, int n, const void* o, int g, const void* f, const void* t, int e) { return refuse_move(c, n, o, g, f, t, e).status; }
+extern "C" int q_size(int i) {
+    return i == 0 ? sizeof(jamhip_kv_pages) : i == 1 ? sizeof(jamhip_tree) : i == 2 ? sizeof(jamhip_tree_path) : sizeof(jamhip_kv_cache);
+}
+"""
+OK, E, U, P = 0, 1, 2, 1 << 20
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    d = tmp_path_factory.mktemp("tree")
+    (d / "t.cpp").write_text(SHIM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{ROOT / 'qxotic_amd' / 'csrc'}", f"-I{ROOT / 'include'}",
+                    str(d / "t.cpp"), "-o", str(d / "t.so")], check=True)
+    return ctypes.CDLL(str(d / "t.so"))
+
+
+def test_seen_keys(lib):
+    """Spans, hulls, single keys and tiles of 64 against the list of keys; words beside the row are never looked at (they are noise here)."""
+    r = random.Random(1)
+    for trial in range(3000):
+        n_words = r.choice([1, 1, 1, 2, 3])
+        base, own = r.choice([0, 0, 5, 70]), r.choice([0, 1, 3, 40, 64, 90, 130])
+        nq = r.choice([0, 1, 2, 7, 63, 64, 65, 64 * n_words, 64 * n_words + 9])
+        first, window = own - nq, r.choice([0, 0, 0, 1, 2, 5, 64, 100])
+        bits = {j for j in range(64 * n_words) if r.random() < r.choice([0.0, 0.1, 0.5, 1.0])}
+        row = T.words([bits], n_words)[0]
+        noise = np.random.default_rng(trial).integers(0, 1 << 63, n_words + 4, dtype=np.int64).view(np.uint64)
+        noise[2:-2] = row
+        ctx = base + max(first, 0)
+        # drafted token j is the sequence's own first + j: those in front of the own ones have no entry
+        have = {j for j in bits if j < min(nq, 64 * n_words) and first + j >= 0}
+        want = list(range(ctx)) + [base + first + j for j in sorted(have)]
+        want = set(want[-window:] if window else want)
+        skip = r.choice([0, 0, base])
+        total = base + own - skip
+        c0 = r.randint(0, max(0, total)) if r.random() < 0.6 else 0
+        c1 = r.randint(c0, max(c0, total)) if r.random() < 0.6 else total
+        want = {k - skip for k in want if c0 <= k - skip < c1}
+        n = max(total, 1)
+        o, sees, tiles = (ctypes.c_int * 4)(), (ctypes.c_int * n)(), (ctypes.c_uint64 * n)()
+        lib.q_span(ctypes.c_void_p(noise.ctypes.data + 16), n_words, base, first, nq, window, skip, c0, c1, n, o, sees, tiles)
+        assert {i for i in range(n) if sees[i]} == want
+        for i in range(n):
+            assert tiles[i] == sum(1 << (k - i) for k in want if i <= k < i + 64), (trial, i)
+        if want:
+            assert (o[2], o[3]) == (min(want), max(want)) and o[0] <= min(want) and o[1] > max(want)
+            assert o[1] <= max(total, 0)
+        else:
+            assert o[2] > o[3]
+
+
+def test_binding_sizes(lib):
+    from qxotic_amd.jam import KvCache, KvPages, Tree, TreePath
+    assert [ctypes.sizeof(t) for t in (KvPages, Tree, TreePath, KvCache)] == [lib.q_size(i) for i in range(4)]
+
+
+def test_refused_pages(lib):
+    from qxotic_amd.jam import KvPages
+    arrays = ("lens", "targets", "base", "held", "n_free", "free_pages", "seq_pages", "lens_out", "held_out", "n_free_out", "status", "q_offsets",
+              "pos", "slots")
+    good = dict(n_seqs=2, n_tokens=3, page_tokens=16, n_pages=9, free_cap=9, ld_seq_pages=4, **{k: P for k in arrays})
+    call = lambda **kw: lib.q_pages(ctypes.byref(KvPages(**{**good, **kw})))   # noqa: E731
+    assert lib.q_pages(None) == E and call() == OK and call(base=None) == OK and call(n_tokens=0, pos=None, slots=None) == OK
+    assert call(n_seqs=0, **{k: None for k in ("lens", "targets", "held", "lens_out", "held_out", "status", "seq_pages")}) == OK
+    for k in arrays:
+        assert k == "base" or call(**{k: None}) == E, k
+    for k in ("n_seqs", "n_tokens", "page_tokens", "n_pages", "free_cap", "ld_seq_pages"):
+        assert call(**{k: -1}) == E, k
+    assert call(page_tokens=0) == E and call(n_seqs=(1 << 20) + 1) == U and call(n_pages=1 << 28) == U and call(n_tokens=(1 << 31) - 1) == U
+
+
+def test_refused_trees(lib):
+    from qxotic_amd.jam import KvCache, Tree, TreePath
+    tree = lambda **kw: Tree(**{**dict(n_tokens=3, n_seqs=2, max_q=2, q_offsets=P, parents=P), **kw})   # noqa: E731
+    call = lambda **kw: lib.q_tree(ctypes.byref(tree(**kw)))   # noqa: E731
+    assert lib.q_tree(None) == E and call() == OK and call(q_offsets=None) == E and call(parents=None) == E
+    assert call(n_tokens=0, q_offsets=None, parents=None) == OK
+    for k in ("n_tokens", "n_seqs", "max_q"):
+        assert call(**{k: -1}) == E, k
+    assert call(n_seqs=(1 << 20) + 1) == U and call(n_tokens=(1 << 31) - 1) == U
+    masks = lambda p, words, q: lib.q_masks(ctypes.c_void_p(p), words, q)   # noqa: E731
+    assert masks(P, 1, 64) == OK and masks(P, 2, 65) == OK
+    assert masks(None, 1, 1) == E and masks(P + 4, 1, 1) == E and masks(P, 0, 0) == E and masks(P, 1, 65) == E and masks(P, -1, 1) == E
+    assert masks(P, 1 << 28, 1) == U
+    good = dict(ld_path=4, path=P, accepted=P, next=P, lens=P, lens_out=P, slots=P, move_from=P, move_to=P)
+    a, b = ctypes.c_void_p(P), ctypes.c_void_p(P)
+    path = lambda a=a, b=b, **kw: lib.q_path(ctypes.byref(tree()), a, b, ctypes.byref(TreePath(**{**good, **kw})))   # noqa: E731
+    assert path() == OK and lib.q_path(ctypes.byref(tree()), a, b, None) == E and path(a=None) == E and path(b=None) == E
+    for k in ("path", "accepted", "next", "lens", "slots", "move_from", "move_to"):
+        assert path(**{k: None}) == E, k
+    assert path(ld_path=-1) == E and path(ld_path=0, path=None) == OK
+    assert path(lens=None, lens_out=None) == OK and path(move_from=None, move_to=None, slots=None) == OK
+    shape = dict(type=8, kv_heads=2, head_dim=64, page_tokens=16, n_pages=4, k=P, v=P)
+    caches = lambda *kw: (KvCache * len(kw))(*(KvCache(**{**shape, **k}) for k in kw))   # noqa: E731
+    move = lambda c, n, o=a, g=1, f=a, t=a, e=1: lib.q_move(c, n, o, g, f, t, e)   # noqa: E731
+    two = caches({}, {"k": 2 * P})
+    assert move(two, 2) == OK and move(None, 1) == E and move(two, -1) == E and move(two, 2, g=-1) == E and move(two, 2, e=-1) == E
+    assert move(two, 2, o=None) == E and move(two, 2, f=None) == E and move(two, 2, t=None) == E and move(two, 2, o=None, f=None, t=None, e=0) == OK
+    for k, v in dict(type=1, kv_heads=1, head_dim=96, page_tokens=8, n_pages=5).items():
+        assert move(caches({}, {k: v}), 2) == E, k
+    assert move(two, 2, g=(1 << 20) + 1) == U and move(two, 2, e=(1 << 31) - 1) == U
+
+
+def test_oracle_resize_restores_its_list():
+    """The definition itself: what one call takes the next gives back, and the list is as it was."""
+    free, table = list(range(20, 9, -1)), [[1, 2, -1, -1], [3, -1, -1, -1], [-1] * 4]
+    lens, held = [20, 5, 0], [2, 1, 0]
+    up, rest = T.resize(16, lens, [40, 33, 17], [0, 0, 0], held, free, table, 100)
+    assert up["status"] == [0, 0, 0] and up["held"] == [3, 3, 2] and len(rest) == len(free) - 5
+    down, back = T.resize(16, up["lens"], lens, [0, 0, 0], up["held"], rest, up["seq_pages"], 100)
+    assert back == free and down["held"] == held and down["lens"] == lens and down["q_offsets"] == [0, 0, 0, 0]
