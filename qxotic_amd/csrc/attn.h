@@ -101,13 +101,20 @@ JAMHIP_DEV int seq_of(const BatchLanes& b, int t) {   // t the same in every lan
     return in ? __ffsll(in) - 1 : -1;
 }
 
-// Row (KvView::row) of key `at` of head `head` of a sequence's prefix and own tokens together.
-JAMHIP_DEV int64_t entry_row(const KvView& c, const SeqInfo& r, int at, int head) {
+// Where key `at` of a sequence's prefix and own tokens together is: its page, as the table has it, and its place in it.
+struct EntryAt {
+    int page, in;
+};
+JAMHIP_DEV EntryAt entry_at(const KvView& c, const SeqInfo& r, int at) {
     const bool shared = at < r.base;
-    const int i = shared ? at : at - r.base, pg = c.page.div(i), in = i - pg * c.page.d;
-    const int p = (shared ? r.prefix : r.own)[pg];
-    return ((int64_t) ((uint32_t) p < (uint32_t) c.n_pages ? p : 0) * c.kv + head) * c.page.d + in;
+    const int i = shared ? at : at - r.base, pg = c.page.div(i);
+    return {(shared ? r.prefix : r.own)[pg], i - pg * c.page.d};
 }
+// Its row (KvView::row) of head `head`.
+JAMHIP_DEV int64_t entry_row(const KvView& c, const EntryAt& e, int head) {
+    return ((int64_t) ((uint32_t) e.page < (uint32_t) c.n_pages ? e.page : 0) * c.kv + head) * c.page.d + e.in;
+}
+JAMHIP_DEV int64_t entry_row(const KvView& c, const SeqInfo& r, int at, int head) { return entry_row(c, entry_at(c, r, at), head); }
 
 // What query token `tok` of a sequence with these SeqInfo values sees (treemask.h).
 JAMHIP_DEV TreeMask tree_mask(const Attn& g, int tok) { return {g.masks + (int64_t) tok * g.mask_words, g.mask_words}; }

@@ -82,6 +82,7 @@ JAMHIP_DEV int wave_min(int v) {   // a butterfly within rows of 16, then the ro
     return min(min(lane_int(v, 0), lane_int(v, 16)), min(lane_int(v, 32), lane_int(v, 48)));
 }
 JAMHIP_DEV int wave_max(int v) { return -wave_min(-v); }
+JAMHIP_DEV int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }   // the same in every lane: a scalar register
 
 // Byte offset of 16-byte chunk c of a key's row. The key's low bits are spread over the chunk's: eight neighbouring keys' equal
 // chunks (the first product's read) fall into eight different 16-byte columns, and so do four neighbouring keys' pairs of
@@ -89,6 +90,10 @@ JAMHIP_DEV int wave_max(int v) { return -wave_min(-v); }
 template <int STRIDE> JAMHIP_DEV int lds_at(int key, int c) {
     return key * STRIDE + ((c ^ ((key & 3) * 2 + ((key >> 2) & 1))) << 4);
 }
+
+// The same, of a chunk a known distance behind another of the row: rows start on 128 bytes, so the low three bits of the distance
+// (which share none with the first chunk's) go in by an exclusive or, the rest by an addition.
+JAMHIP_DEV int lds_step(int at, int chunks) { return (at ^ ((chunks & 7) << 4)) + (chunks >> 3) * 128; }
 
 // A lane's 8 elements of the query row for each of STEPS products, element `at(step)` and 4 on, then `at4(step)` and 4 on: hi and
 // lo halves of the row scaled by a power of two. Returns f: a score in powers of two is f times the product.
@@ -190,19 +195,21 @@ template <int ROWS> JAMHIP_DEV bool attn_row_set(const AttnArgs& a, int tile, Ro
 }
 
 // ---- a lane's column: a row and the keys that it sees, those of the workgroup's run of chunk keys
+struct Seen {
+    int tok, head, live;
+    int see_lo, see_n;   // key sees: (unsigned) (key - see_lo) <= see_n
+    TreeSpan span;       // of a drafted tree's token: what it sees of the run
+};
 struct Column {
-    int tok, head;
-    bool live;
-    int see_lo, see_n;     // key sees: (unsigned) (key - see_lo) <= see_n
+    Seen seen;
     int lo, hi;            // the wave's first and last key that a row sees
     int all_lo, all_hi;    // between these every live row sees all
-    TreeSpan span;         // of a drafted tree's token: what it sees of the run
-    TreeMask mask;
 };
 
 template <bool TREE> JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowSet& w, int r, int kvh, int split) {
     const Attn& g = a.g;
-    Column c;
+    Column col;
+    Seen& c = col.seen;
     const int rr = min(r, w.n_rows - 1), total = w.s.base + w.s.len;
     c.tok = w.t_first + g.grp.div(rr);
     c.head = kvh * g.grp.d + (rr - (c.tok - w.t_first) * g.grp.d);
@@ -233,42 +240,44 @@ template <bool TREE> JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowS
     }
     const int c0 = split * a.part.chunk;
     if constexpr (TREE) {   // the context's keys, and the drafted ones' by their bits
-        c.mask = tree_mask(g, c.tok);
+        const TreeMask mask = tree_mask(g, c.tok);
         // the window counts the whole context's keys: in mode 2 positions are among the own ones
         const int skip = a.part.mode == 2 ? w.base_all : 0;
-        c.span = span_cut(tree_span(c.mask, w.s.base + skip, s_first, s_nq, g.window), skip, c0, min(c0 + a.part.chunk, total));
-        const TreeHull h = span_hull(c.mask, c.span);
+        c.span = span_cut(tree_span(mask, w.s.base + skip, s_first, s_nq, g.window), skip, c0, min(c0 + a.part.chunk, total));
+        const TreeHull h = span_hull(mask, c.span);
         const bool some = c.live && h.lo <= h.hi, ctx = c.live && c.span.ctx_lo < c.span.ctx_hi;
         c.see_lo = INT32_MAX, c.see_n = 0;
-        c.lo = wave_min(some ? h.lo : INT32_MAX), c.hi = wave_max(some ? h.hi : -1);
-        c.all_lo = wave_max(c.live ? (ctx ? c.span.ctx_lo : INT32_MAX) : -1);
-        c.all_hi = wave_min(c.live ? (ctx ? c.span.ctx_hi - 1 : -1) : INT32_MAX);
-        return c;
+        col.lo = uniform(wave_min(some ? h.lo : INT32_MAX)), col.hi = uniform(wave_max(some ? h.hi : -1));
+        col.all_lo = uniform(wave_max(c.live ? (ctx ? c.span.ctx_lo : INT32_MAX) : -1));
+        col.all_hi = uniform(wave_min(c.live ? (ctx ? c.span.ctx_hi - 1 : -1) : INT32_MAX));
+        return col;
     }
     const int k_lo = max(c0, g.window > 0 ? pos - g.window + 1 : 0), k_hi = min(min(total, c0 + a.part.chunk) - 1, pos);   // first and last
     const bool some = c.live && k_lo <= k_hi;
     c.see_lo = some ? k_lo : INT32_MAX, c.see_n = some ? k_hi - k_lo : 0;
-    c.lo = wave_min(some ? k_lo : INT32_MAX), c.hi = wave_max(some ? k_hi : -1);
-    c.all_lo = wave_max(c.live ? (some ? k_lo : INT32_MAX) : -1), c.all_hi = wave_min(c.live ? (some ? k_hi : -1) : INT32_MAX);
-    return c;
+    col.lo = uniform(wave_min(some ? k_lo : INT32_MAX)), col.hi = uniform(wave_max(some ? k_hi : -1));
+    col.all_lo = uniform(wave_max(c.live ? (some ? k_lo : INT32_MAX) : -1)), col.all_hi = uniform(wave_min(c.live ? (some ? k_hi : -1) : INT32_MAX));
+    return col;
 }
 
 // ---- the softmax's step: a tile's scores sc (of ST products' accumulators) become weights; o and l follow the maximum
 template <typename M, int ST, int DT, int NC, bool TREE, typename ACC>
-JAMHIP_DEV void attn_weights(ACC (&sc)[ST], ACC (&o)[DT], float& m, float& l, float f, const Column& c, int kw, int part) {
+JAMHIP_DEV void attn_weights(ACC (&sc)[ST], ACC (&o)[DT], float& m, float& l, float f, const Column& c, const Seen& seen, const Attn& g, int kw,
+                             int part) {
     if (TREE && (kw < c.all_lo || kw + ST * NC - 1 > c.all_hi)) {
-        const uint64_t sees = span_tile(c.mask, c.span, kw) >> (4 * part);   // M::row(k, part) = M::row(k, 0) + 4 · part
+        const uint64_t sees = span_tile(tree_mask(g, seen.tok), seen.span, kw) >> (4 * part);   // M::row(k, part) = M::row(k, 0) + 4 · part
 #pragma unroll
         for (int i = 0; i < ST; i++)
 #pragma unroll
             for (int k = 0; k < M::N; k++)
                 if (!(sees >> (i * NC + M::row(k, 0)) & 1)) sc[i][k] = -__builtin_inff();
     } else if (!TREE && (kw < c.all_lo || kw + ST * NC - 1 > c.all_hi)) {
+        const int see_lo = seen.see_lo, see_n = seen.see_n;
 #pragma unroll
         for (int i = 0; i < ST; i++)
 #pragma unroll
             for (int k = 0; k < M::N; k++)
-                if ((unsigned) (kw + i * NC + M::row(k, part) - c.see_lo) > (unsigned) c.see_n) sc[i][k] = -__builtin_inff();
+                if ((unsigned) (kw + i * NC + M::row(k, part) - see_lo) > (unsigned) see_n) sc[i][k] = -__builtin_inff();
     }
     float top = sc[0][0];
 #pragma unroll
@@ -309,27 +318,29 @@ template <int NC, int ST, typename ACC> JAMHIP_DEV void weight_halves(const ACC 
     }
 }
 
-// O += Vᵀ · P for product u, the values at `lv` in rows of STRIDE bytes from key kb on: 16 lanes read 4 keys of 16 elements and get
-// 4 keys of their element, twice, which is the keys' order in the weights.
-template <int NC, int DT, int STRIDE, typename M, typename ACC>
-JAMHIP_DEV void add_values(ACC (&o)[DT], const uint8_t* lv, int kb, int u, half8_t ph, half8_t pl) {
+// Element tile d of Vᵀ for product u, the values at `lv` in rows of STRIDE bytes: 16 lanes read 4 keys of 16 elements and get 4 keys of
+// their element, twice, which is the keys' order in the weights.
+template <int NC, int STRIDE, typename M> JAMHIP_DEV half8_t value_tile(const uint8_t* lv, int d, int u) {
     const int lane = threadIdx.x & 63, part = lane / NC, in = lane % 16, sub = NC == 32 ? (lane / 16) % 2 : 0;
-    const int key = kb + u * M::DEPTH + 4 * part + in / 4;
+    const int first = lds_at<STRIDE>(4 * part + in / 4, 2 * sub + in % 4 / 2) + in % 2 * 8;   // of element tile 0
+    auto at = [&](int k) {   // k is a multiple of 8 keys behind the lane's: the same columns
+        const uint8_t* p = lv + lds_step(first, d * NC / 8) + k * STRIDE;
+        const short4_t w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4_t*) (uintptr_t) (__attribute__((address_space(3))) const uint8_t*) p);
+        return __builtin_bit_cast(half4_t, w);
+    };
+    return join_half(at(u * M::DEPTH), at(u * M::DEPTH + M::DEPTH / 2));
+}
+
+// O += Vᵀ · P for product u.
+template <int NC, int DT, int STRIDE, typename M, typename ACC>
+JAMHIP_DEV void add_values(ACC (&o)[DT], const uint8_t* lv, int u, half8_t ph, half8_t pl) {
     constexpr int PAIR = NC == 32 ? 2 : 1;   // two products between hi and lo of one sum, where there are registers for them
 #pragma unroll
     for (int d0 = 0; d0 < DT; d0 += PAIR) {
         half8_t v[PAIR];
 #pragma unroll
-        for (int i = 0; i < PAIR && d0 + i < DT; i++) {
-            const int e0 = (d0 + i) * NC + sub * 16 + 4 * (in % 4);
-            auto at = [&](int k) {
-                const uint8_t* p = lv + lds_at<STRIDE>(k, e0 / 8) + e0 % 8 * 2;
-                const short4_t w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) short4_t*) (uintptr_t) (__attribute__((address_space(3))) const uint8_t*) p);
-                return __builtin_bit_cast(half4_t, w);
-            };
-            v[i] = join_half(at(key), at(key + M::DEPTH / 2));
-        }
+        for (int i = 0; i < PAIR && d0 + i < DT; i++) v[i] = value_tile<NC, STRIDE, M>(lv, d0 + i, u);
 #pragma unroll
         for (int i = 0; i < PAIR && d0 + i < DT; i++) o[d0 + i] = M::mma(v[i], ph, o[d0 + i]);
 #pragma unroll
@@ -342,15 +353,16 @@ JAMHIP_DEV void add_values(ACC (&o)[DT], const uint8_t* lv, int kb, int u, half8
 struct KeyAt {
     int64_t code, scale;
 };
-template <int TYPE, int D> JAMHIP_DEV KeyAt key_at(const KvView& c, const SeqInfo& s, int at, int head) {
-    const int64_t row = entry_row(c, s, at, head);
+template <int TYPE, int D> JAMHIP_DEV KeyAt key_at(const KvView& c, const EntryAt& e, int head) {
+    const int64_t row = entry_row(c, e, head);
     return {row * kv_row_bytes(TYPE, D), c.scale_off + row * (D / 32) * 2};
 }
 
-// ---- 16 bytes of codes of a row into shared memory as f16
-template <int TYPE, int STRIDE> JAMHIP_DEV void put_unit(uint8_t* plane, const uint4_t& w, _Float16 sc, int key, int c) {
+// ---- 16 bytes of codes of a row into shared memory as f16, from `at` on: unit_at of the key and the unit
+template <int TYPE, int STRIDE> JAMHIP_DEV int unit_at(int key, int unit) { return lds_at<STRIDE>(key, unit * (unit_elems<TYPE>() / 8)); }
+template <int TYPE> JAMHIP_DEV void put_unit(uint8_t* plane, const uint4_t& w, _Float16 sc, int at) {
     if constexpr (TYPE == F16) {
-        *reinterpret_cast<uint4_t*>(plane + lds_at<STRIDE>(key, c)) = w;
+        *reinterpret_cast<uint4_t*>(plane + at) = w;
     } else {
         const half2_t scale = {sc, sc};
         half2_t h[16];
@@ -365,7 +377,7 @@ template <int TYPE, int STRIDE> JAMHIP_DEV void put_unit(uint8_t* plane, const u
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const uint4_t v = {as_u32(h[4 * i]), as_u32(h[4 * i + 1]), as_u32(h[4 * i + 2]), as_u32(h[4 * i + 3])};
-            *reinterpret_cast<uint4_t*>(plane + lds_at<STRIDE>(key, c * N + i)) = v;
+            *reinterpret_cast<uint4_t*>(plane + lds_step(at, i)) = v;
         }
     }
 }
@@ -381,17 +393,17 @@ JAMHIP_DEV unsigned long long attn_emit(const AttnArgs& a, const Column& c, cons
     float* dst;
     if (a.part.direct) {
         if (g.sinks != nullptr) {
-            const float x = g.sinks[c.head] * LOG2E, now = fmaxf(m, x);
+            const float x = g.sinks[c.seen.head] * LOG2E, now = fmaxf(m, x);
             const float keep = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
             l = l * keep + (now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(x - now + WEIGHT_EXP));
             scale = keep;
         }
         scale = l == 0.0f ? 0.0f : scale / l;
-        dst = g.out + (int64_t) c.tok * g.ldo + (int64_t) c.head * D;
+        dst = g.out + (int64_t) c.seen.tok * g.ldo + (int64_t) c.seen.head * D;
     } else {
-        const int64_t n = (int64_t) g.n_tokens * g.heads, at = (int64_t) (a.part.slot0 + split) * n + (int64_t) c.tok * g.heads + c.head;
+        const int64_t n = (int64_t) g.n_tokens * g.heads, at = (int64_t) (a.part.slot0 + split) * n + (int64_t) c.seen.tok * g.heads + c.seen.head;
         dst = a.acc + at * D;
-        if (c.live && part == 0 && turn == 0) a.ml[at] = make_float2(m, l);
+        if (c.seen.live && part == 0 && turn == 0) a.ml[at] = make_float2(m, l);
     }
     const bool al = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
     bool bad = false;
@@ -407,7 +419,7 @@ JAMHIP_DEV unsigned long long attn_emit(const AttnArgs& a, const Column& c, cons
                 bad |= !(fabsf(v[e]) < __builtin_inff());
             }
             float* p = dst + dt * NC + M::row(k, part);
-            if (c.live) {
+            if (c.seen.live) {
                 if (al) {
                     *reinterpret_cast<float4_t*>(p) = v;
                 } else {
@@ -417,7 +429,7 @@ JAMHIP_DEV unsigned long long attn_emit(const AttnArgs& a, const Column& c, cons
             }
         }
     }
-    unsigned long long again = a.part.direct ? __ballot(bad && c.live) : 0;
+    unsigned long long again = a.part.direct ? __ballot(bad && c.seen.live) : 0;
 #pragma unroll
     for (int k = NC; k < 64; k <<= 1) again |= again >> k;
     return again & ((1ull << NC) - 1);

@@ -34,6 +34,7 @@ template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256, D <
     __shared__ __align__(16) uint8_t lds[2 * T::PLANE];
     __shared__ __align__(16) KeyAt rows[2][KEYS];
     __shared__ int range[2][4];
+    __shared__ Seen seen[4][NC];   // looked at for tiles that some row does not see whole: not kept in registers
     __shared__ float redo[4][ATTN_ROW_FLOATS];
     const Attn& g = a.g;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -46,14 +47,15 @@ template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256, D <
     const int tile = rows_last ? b / a.part.splits : b % a.part.tiles, split = rows_last ? b % a.part.splits : b / a.part.tiles;
     RowSet w;
     if (!attn_row_set<T::ROWS>(a, tile, &w)) return;
-    const Column c = attn_column<TREE>(a, w, w.r0 + wave * NC + col, kvh, split);
+    Column c = attn_column<TREE>(a, w, w.r0 + wave * NC + col, kvh, split);
+    seen[wave][col] = c.seen;   // both parts of a column the same
     if (lane == 0) range[0][wave] = c.lo, range[1][wave] = c.hi;
     half8_t qh[T::STEPS], ql[T::STEPS];
-    const float f = load_query<NC>(g.q + (int64_t) c.tok * g.ldq + (int64_t) c.head * D, g.scale, qh, ql,
+    const float f = load_query<NC>(g.q + (int64_t) c.seen.tok * g.ldq + (int64_t) c.seen.head * D, g.scale, qh, ql,
                                    [&](int st, int j) { return st * M::DEPTH + part * 8 + j; });
     __syncthreads();
-    const int lo = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3]));
-    const int hi = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3])) + 1;   // one past the last
+    const int lo = uniform(min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3])));
+    const int hi = uniform(max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]))) + 1;   // one past the last
 
     acc_t o[T::DT];
 #pragma unroll
@@ -65,22 +67,32 @@ template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256, D <
     uint4_t kr[T::PER], vr[T::PER];
     _Float16 ks[T::PER] = {}, vs[T::PER] = {};
     // past the last key it stands for that one: no load is behind a branch, and nothing that no row sees comes in
-    auto row_of = [&](int at) { return key_at<TYPE, D>(g.cache, w.s, min(at, hi - 1), kvh); };
+    auto entry_of = [&](int at) { return entry_at(g.cache, w.s, min(at, hi - 1)); };
+    auto row_of = [&](int at) { return key_at<TYPE, D>(g.cache, entry_of(at), kvh); };
+    // unit i of a thread: where the units of 256 threads are whole rows, 8 or a multiple apart, its place follows from the first one's
+    constexpr bool EVEN = 256 % T::UPK == 0 && 256 / T::UPK % 8 == 0;
+    auto key_of = [&](int i) { return EVEN ? tid / T::UPK + i * (256 / T::UPK) : (tid + 256 * i) / T::UPK; };
+    auto place_of = [&](int i) {
+        return EVEN ? unit_at<TYPE, T::STRIDE>(tid / T::UPK, tid % T::UPK) + i * (256 / T::UPK) * T::STRIDE
+                    : unit_at<TYPE, T::STRIDE>(key_of(i), (tid + 256 * i) % T::UPK);
+    };
     auto fetch = [&](const KeyAt* rw) {
 #pragma unroll
         for (int i = 0; i < T::PER; i++) {
-            const int u = tid + 256 * i, key = u / T::UPK, ch = u % T::UPK;
-            const KeyAt row = rw[T::UNITS % 256 == 0 ? key : min(key, KEYS - 1)];
-            kr[i] = *reinterpret_cast<const uint4_t*>(g.cache.k + row.code + ch * 16);
-            vr[i] = *reinterpret_cast<const uint4_t*>(g.cache.v + row.code + ch * 16);
+            const KeyAt row = rw[T::UNITS % 256 == 0 ? key_of(i) : min(key_of(i), KEYS - 1)];
+            int ch = EVEN ? tid % T::UPK : (tid + 256 * i) % T::UPK;
+            asm volatile("" : "+v"(ch));   // added here: four addresses kept for it over the loop are eight registers
+            kr[i] = *reinterpret_cast<const uint4_t*>(g.cache.k + (row.code + ch * 16));
+            vr[i] = *reinterpret_cast<const uint4_t*>(g.cache.v + (row.code + ch * 16));
             if constexpr (TYPE != F16) {
-                ks[i] = *reinterpret_cast<const _Float16*>(g.cache.k + row.scale + ch * T::EPU / 32 * 2);
-                vs[i] = *reinterpret_cast<const _Float16*>(g.cache.v + row.scale + ch * T::EPU / 32 * 2);
+                ks[i] = *reinterpret_cast<const _Float16*>(g.cache.k + (row.scale + ch * T::EPU / 32 * 2));
+                vs[i] = *reinterpret_cast<const _Float16*>(g.cache.v + (row.scale + ch * T::EPU / 32 * 2));
             }
         }
     };
     uint8_t* const lk = lds;
     uint8_t* const lv = lds + T::PLANE;
+    const int own = lds_at<T::STRIDE>(col, part);   // the lane's first chunk of a tile's keys
     if (lo < hi) {
         if (tid < KEYS) rows[0][tid] = row_of(lo + tid), rows[1][tid] = row_of(lo + KEYS + tid);
         __syncthreads();
@@ -91,16 +103,16 @@ template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256, D <
         __syncthreads();   // the tile before is read; rows[buf] is the next one's
 #pragma unroll
         for (int i = 0; i < T::PER; i++) {
-            const int u = tid + 256 * i, key = u / T::UPK, ch = u % T::UPK;
-            if (T::UNITS % 256 == 0 || u < T::UNITS) {
-                put_unit<TYPE, T::STRIDE>(lk, kr[i], ks[i], key, ch);
-                put_unit<TYPE, T::STRIDE>(lv, vr[i], vs[i], key, ch);
+            if (T::UNITS % 256 == 0 || tid + 256 * i < T::UNITS) {
+                put_unit<TYPE>(lk, kr[i], ks[i], place_of(i));
+                put_unit<TYPE>(lv, vr[i], vs[i], place_of(i));
             }
         }
-        KeyAt after = {};
+        // the page of the next but one's keys is asked for first and looked at last: loads come back in their order
+        EntryAt after = {};
         if (k0 + KEYS < hi) {
+            if (tid < KEYS) after = entry_of(k0 + 2 * KEYS + tid);
             fetch(rows[buf]);
-            if (tid < KEYS) after = row_of(k0 + 2 * KEYS + tid);
         }
         __syncthreads();
         if (k0 <= c.hi && k0 + KEYS > c.lo) {
@@ -109,30 +121,58 @@ template <int TYPE, int D, bool TREE> __global__ void __launch_bounds__(256, D <
             for (int i = 0; i < T::ST; i++)
 #pragma unroll
                 for (int k = 0; k < M::N; k++) sc[i][k] = 0.0f;
+            half8_t x[2][T::ST];   // a step's keys are on their way while the step before is multiplied
+            auto keys_of = [&](int st) {
 #pragma unroll
-            for (int st = 0; st < T::STEPS; st++) {
-                half8_t x[T::ST];
+                for (int i = 0; i < T::ST; i++)
+                    x[st % 2][i] = *reinterpret_cast<const half8_t*>(lk + lds_step(own, st * 2) + i * NC * T::STRIDE);
+            };
+            __builtin_amdgcn_s_setprio(1);
+            keys_of(0);
+            __builtin_amdgcn_sched_group_barrier(0x100, T::ST, 0);
+            unroll<0, T::STEPS>([&](auto step) {
+                constexpr int st = decltype(step)::value;
+                if constexpr (st + 1 < T::STEPS) keys_of(st + 1);
 #pragma unroll
-                for (int i = 0; i < T::ST; i++) x[i] = *reinterpret_cast<const half8_t*>(lk + lds_at<T::STRIDE>(i * NC + col, st * 2 + part));
+                for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[st % 2][i], qh[st], sc[i]);
 #pragma unroll
-                for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], qh[st], sc[i]);
+                for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[st % 2][i], ql[st], sc[i]);
+                if constexpr (st + 1 < T::STEPS) __builtin_amdgcn_sched_group_barrier(0x100, T::ST, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * T::ST, 0);
+            });
+            __builtin_amdgcn_s_setprio(0);
+            attn_weights<M, T::ST, T::DT, NC, TREE>(sc, o, m, l, f, c, seen[wave][col], a.g, k0, part);
+            constexpr int PAIRS = (T::DT + 1) / 2, ALL = KEYS / M::DEPTH * PAIRS;   // pairs of element tiles, over all products
+            half8_t v[2][2], ph[2], pl[2];
+            auto values_of = [&](int n) {
 #pragma unroll
-                for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], ql[st], sc[i]);
-            }
-            attn_weights<M, T::ST, T::DT, NC, TREE>(sc, o, m, l, f, c, k0, part);
+                for (int i = 0; i < 2; i++)
+                    if (2 * (n % PAIRS) + i < T::DT) v[n % 2][i] = value_tile<NC, T::STRIDE, M>(lv, 2 * (n % PAIRS) + i, n / PAIRS);
+            };
+            weight_halves<NC>(sc, 0, ph[0], pl[0]);
+            __builtin_amdgcn_s_setprio(1);
+            values_of(0);
+            unroll<0, ALL>([&](auto step) {
+                constexpr int n = decltype(step)::value, u = n / PAIRS, d = 2 * (n % PAIRS), width = d + 1 < T::DT ? 2 : 1;
+                constexpr bool more = n + 1 < ALL;
+                if constexpr (more) values_of(n + 1);
+                if constexpr (more && (n + 1) % PAIRS == 0) weight_halves<NC>(sc, u + 1, ph[(u + 1) % 2], pl[(u + 1) % 2]);
 #pragma unroll
-            for (int u = 0; u < KEYS / M::DEPTH; u++) {
-                half8_t ph, pl;
-                weight_halves<NC>(sc, u, ph, pl);
-                add_values<NC, T::DT, T::STRIDE, M>(o, lv, 0, u, ph, pl);
-            }
+                for (int i = 0; i < width; i++) o[d + i] = M::mma(v[n % 2][i], ph[u % 2], o[d + i]);
+#pragma unroll
+                for (int i = 0; i < width; i++) o[d + i] = M::mma(v[n % 2][i], pl[u % 2], o[d + i]);
+                if constexpr (more) __builtin_amdgcn_sched_group_barrier(0x100, (n + 1) % PAIRS * 2 + 1 < T::DT ? 4 : 2, 1);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * width, 1);
+            });
+            __builtin_amdgcn_s_setprio(0);
         }
-        if (tid < KEYS) rows[buf ^ 1][tid] = after;   // read for the tile before this one; now the next but one's
+        if (tid < KEYS) rows[buf ^ 1][tid] = key_at<TYPE, D>(g.cache, after, kvh);   // read for the tile before this one; now the next but one's
     }
     l = column_sum<NC>(l);
+    c.seen = seen[wave][col];
     for (unsigned long long again = attn_emit<D, NC, T::DT, 1, M>(a, c, o, m, l, split, 0); again; again &= again - 1) {
         const int k = __ffsll(again) - 1;
-        attn_row<TYPE, TREE>(g, __builtin_amdgcn_readlane(c.tok, k), __builtin_amdgcn_readlane(c.head, k), redo[wave]);
+        attn_row<TYPE, TREE>(g, __builtin_amdgcn_readlane(c.seen.tok, k), __builtin_amdgcn_readlane(c.seen.head, k), redo[wave]);
     }
 }
 

@@ -138,7 +138,7 @@ template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(
     const int lo = c.lo, hi = c.hi + 1;   // the same in every wave
 
     half8_t qh[T::STEPS], ql[T::STEPS];
-    const float f = load_query<NC>(g.q + (int64_t) c.tok * g.ldq + (int64_t) c.head * D, g.scale, qh, ql,
+    const float f = load_query<NC>(g.q + (int64_t) c.seen.tok * g.ldq + (int64_t) c.seen.head * D, g.scale, qh, ql,
                                    [&](int st, int j) { return T::K::element(st, part, j); });
 
     acc_t o[T::DT];
@@ -154,7 +154,8 @@ template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(
     uint4_t vr[T::PER];
     _Float16 vs[T::PER] = {};
     // past the last key it stands for that one: no load is behind a branch, and nothing that no row sees comes in
-    auto row_of = [&](int at) { return key_at<TYPE, D>(g.cache, w.s, min(at, hi - 1), kvh); };
+    auto entry_of = [&](int at) { return entry_at(g.cache, w.s, min(at, hi - 1)); };
+    auto row_of = [&](int at) { return key_at<TYPE, D>(g.cache, entry_of(at), kvh); };
     auto sync = [] { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
     auto fetch_k = [&](const KeyAt* r) {
 #pragma unroll
@@ -181,9 +182,12 @@ template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(
 #pragma unroll
         for (int i = 0; i < T::PER; i++) {
             const int u = lane + 64 * i;
-            if (T::UNITS % 64 == 0 || u < T::UNITS) put_unit<TYPE, T::STRIDE>(lv, vr[i], vs[i], u / T::UPK, u % T::UPK);
+            if (T::UNITS % 64 == 0 || u < T::UNITS) put_unit<TYPE>(lv, vr[i], vs[i], unit_at<TYPE, T::STRIDE>(u / T::UPK, u % T::UPK));
         }
         const bool more = k0 + step < hi;
+        // the page of the next but one's keys is asked for first and looked at last: loads come back in their order
+        EntryAt after = {};
+        if (lane < T::KEYS && k0 + 2 * step < hi) after = entry_of(k0 + 2 * step + lane);
         if (more) fetch_v(rw[buf]);
         acc_t sc[T::ST];
 #pragma unroll
@@ -199,20 +203,16 @@ template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(
 #pragma unroll
             for (int i = 0; i < T::ST; i++) sc[i] = M::mma(x[i], ql[decltype(st)::value], sc[i]);
         });
-        KeyAt after = {};
-        if (more) {
-            fetch_k(rw[buf]);
-            if (lane < T::KEYS && k0 + 2 * step < hi) after = row_of(k0 + 2 * step + lane);
-        }
-        attn_weights<M, T::ST, T::DT, NC, TREE>(sc, o, m, l, f, c, k0, part);
+        if (more) fetch_k(rw[buf]);
+        attn_weights<M, T::ST, T::DT, NC, TREE>(sc, o, m, l, f, c, c.seen, a.g, k0, part);
         sync();   // the values are in shared memory
 #pragma unroll
         for (int u = 0; u < T::KEYS / M::DEPTH; u++) {
             half8_t ph, pl;
             weight_halves<NC>(sc, u, ph, pl);
-            add_values<NC, T::DT, T::STRIDE, M>(o, lv, 0, u, ph, pl);
+            add_values<NC, T::DT, T::STRIDE, M>(o, lv, u, ph, pl);
         }
-        if (lane < T::KEYS) rw[buf ^ 1][lane] = after;
+        if (lane < T::KEYS) rw[buf ^ 1][lane] = key_at<TYPE, D>(g.cache, after, kvh);
         sync();   // and read, before the next tile's take their place
     }
 
@@ -255,7 +255,7 @@ template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(
     __syncthreads();   // a row that one wave finds not finite is whole before it is written again
     for (; again; again &= again - 1) {
         const int k = __ffsll(again) - 1;
-        attn_row<TYPE, TREE>(g, __builtin_amdgcn_readlane(c.tok, k), __builtin_amdgcn_readlane(c.head, k), redo[wave]);
+        attn_row<TYPE, TREE>(g, __builtin_amdgcn_readlane(c.seen.tok, k), __builtin_amdgcn_readlane(c.seen.head, k), redo[wave]);
     }
 }
 
