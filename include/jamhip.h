@@ -403,7 +403,7 @@ typedef struct {
 /* Every sequence gets ceil(target / page_tokens) pages. First the pages that are too many go back to the free list, from the last sequence
  * to the first, each one's last page first; then the sequences take theirs off the list's end, in their order. A sequence that does not
  * fit (the list is empty, its row is full, or its tokens pass n_tokens) is refused, and so is every one behind it that would grow: they
- * keep their pages and lengths. Giving back what the call before took leaves the list as it was. A sequence's new tokens, max(0,
+ * keep their lengths, and their pages but for those that even their targets do not need. Giving back what the call before took leaves the list as it was. A sequence's new tokens, max(0,
  * target - len) of them, are rows q_offsets[s] on of the batch, refused or not (q_offsets stop at n_tokens); row i of them has the
  * position base + len + i and the slot of its place, -1 where the sequence was refused. Rows behind the last sequence's get slot -1 and
  * position 0. n_seqs at most 2^20, n_pages * page_tokens below 2^31 (else JAMHIP_EUNSUPPORTED). */

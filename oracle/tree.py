@@ -24,7 +24,7 @@ def resize(page, lens, targets, base, held, free, table, n_tokens):
             for c in range(held[s], need[s]):
                 table[s][c] = free.pop()
         out["lens"].append(lens[s] if refused else targets[s])
-        out["held"].append(held[s] if refused else need[s])
+        out["held"].append(min(held[s], need[s]) if refused else need[s])
         out["status"].append(int(refused))
         out["q_offsets"].append(min(rows, n_tokens))
         for p in range(lens[s], lens[s] + min(new, n_tokens)):

@@ -53,7 +53,8 @@ inline int attn_splits(int cfg, int64_t groups, int keys, int longest, int* chun
     return up_div(tiles, per);
 }
 
-inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, int n_prefixes, int max_q, int max_seq, int max_prefix) {
+inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, int n_prefixes, int max_q, int max_seq, int max_prefix,
+                          bool tree = false) {
     AttnPlan p{};
     bool fits = true;
     const int64_t rows = (int64_t) max_q * grp;
@@ -72,7 +73,9 @@ inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, in
         p.slots += a.splits;
         fits = fits && tiles <= INT32_MAX / kv / a.splits;
     };
-    const int cfg = attn_cfg(rows, dim);
+    // Trees of more rows than that whose 128-row tiles would leave most of the chip idle, however their keys are split
+    const bool few = tree && dim <= ATTN_WIDE_DIM && (rows + 127) / 128 * n_seqs * kv * ((max_seq + (int64_t) max_prefix + 127) / 128) < 256;
+    const int cfg = few && rows > 16 ? 1 : attn_cfg(rows, dim);
     const int64_t per = (rows + attn_rows(cfg) - 1) / attn_rows(cfg);
     if (!grouped) {
         add(0, cfg, per * n_seqs, per * n_seqs, max_seq + max_prefix);

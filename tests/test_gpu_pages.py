@@ -79,7 +79,8 @@ def make(r, n, page, most, grow, spare=4, slack=0, apart=False, shrink=0.3, base
 
 @pytest.mark.parametrize("apart", [False, True])
 @pytest.mark.parametrize("n,page,most,grow", [(1, 16, 0, 1), (1, 16, 40, 33), (3, 1, 9, 5), (64, 16, 300, 32), (65, 7, 90, 100), (200, 64, 1000, 1),
-                                              (1023, 16, 100, 40), (1024, 16, 100, 40), (1025, 32, 64, 70), (2500, 16, 50, 9), (2, 16, 100, 40000)])
+                                              (1023, 16, 100, 40), (1024, 16, 100, 40), (1025, 32, 64, 70), (2500, 16, 50, 9), (2, 16, 100, 40000), (700, 16, 6000, 30),
+                                              (1, 1, 5, 1100000)])
 def test_resize(hip, n, page, most, grow, apart):
     say("resize", n, page, most, grow, apart)
     r = np.random.default_rng(n + page)
@@ -108,6 +109,21 @@ def test_resize_refusals_on_the_device(hip, n):
     p.d["targets"][n // 2] = p.host["targets"][n // 2]
     out, _ = p.run(hip).check()
     assert out["status"][n // 2] == 1
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("n", [3, 1500])
+def test_resize_refused_with_pages_to_spare(hip, n, apart):
+    """A refused sequence that held more pages than its target needs: those are on the list, once, and it holds the rest."""
+    r = np.random.default_rng(n)
+    lens, targets, held = [30] * n, [33] * n, [int(v) for v in r.integers(2, 7, n)]
+    order = list(r.permutation(8 * n))
+    table = [[int(order.pop()) for _ in range(h)] + [-5] * (8 - h) for h in held]
+    p = Pool(lens, targets, held, table, [], 16, 8 * n, 3 * (n // 2), apart=apart)
+    out, free = p.run(hip).check()
+    assert sum(out["status"]) > 0
+    kept = [row[c] for row, h in zip(out["seq_pages"], out["held"]) for c in range(h)]
+    assert len(set(kept + free)) == len(kept) + len(free)   # no page twice
 
 
 def test_resize_nothing_and_extremes(hip):
