@@ -244,10 +244,11 @@ template <bool TREE> JAMHIP_DEV Column attn_column(const AttnArgs& a, const RowS
         // the window counts the whole context's keys: in mode 2 positions are among the own ones
         const int skip = a.part.mode == 2 ? w.base_all : 0;
         c.span = span_cut(tree_span(mask, w.s.base + skip, s_first, s_nq, g.window), skip, c0, min(c0 + a.part.chunk, total));
-        const TreeHull h = span_hull(mask, c.span);
-        const bool some = c.live && h.lo <= h.hi, ctx = c.live && c.span.ctx_lo < c.span.ctx_hi;
+        // the drafted keys as far as there are bits, set or not: looking at them here would be a round of loads before the pages' and codes'
+        const int k_lo = span_lo(c.span), k_hi = span_hi(c.span) - 1;
+        const bool some = c.live && k_lo <= k_hi, ctx = c.live && c.span.ctx_lo < c.span.ctx_hi;
         c.see_lo = INT32_MAX, c.see_n = 0;
-        col.lo = uniform(wave_min(some ? h.lo : INT32_MAX)), col.hi = uniform(wave_max(some ? h.hi : -1));
+        col.lo = uniform(wave_min(some ? k_lo : INT32_MAX)), col.hi = uniform(wave_max(some ? k_hi : -1));
         col.all_lo = uniform(wave_max(c.live ? (ctx ? c.span.ctx_lo : INT32_MAX) : -1));
         col.all_hi = uniform(wave_min(c.live ? (ctx ? c.span.ctx_hi - 1 : -1) : INT32_MAX));
         return col;

@@ -257,29 +257,21 @@ __global__ void __launch_bounds__(FILL) kv_slots_kernel(Pages g) {
 }
 
 // ---- entries moved
-// A workgroup moves one group's entries in one cache: a thread holds the same piece of every entry, so that the entries of a group go in their
-// order without a barrier between them.
+// A workgroup moves one group's entries in one cache: a thread holds the same pieces of every entry, so that the entries of a group go in their
+// order without a barrier between them. Pieces are 16 bytes of codes, and scales one by one (their rows are 2, 4, 6 bytes and so on): keys'
+// codes, values' codes, keys' scales, values' scales, numbered through, so that all of an entry is loaded before the first is stored.
 constexpr int BATCH = 4;
 
-template <typename U> JAMHIP_DEV void move_pieces(uint8_t* buf, int64_t plane, int pieces, int per_head, const KvView& c, const int* pf,
-                                                  const int* at_f, const int* pt, const int* at_t, int n) {
-    for (int u = threadIdx.x; u < pieces; u += blockDim.x) {
-        const int head = u / per_head, at = u - head * per_head;
-        U v[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; i++)
-            if (i < n) v[i] = reinterpret_cast<const U*>(buf + plane)[(((int64_t) pf[i] * c.kv + head) * c.page.d + at_f[i]) * per_head + at];
-#pragma unroll
-        for (int i = 0; i < BATCH; i++)
-            if (i < n) reinterpret_cast<U*>(buf + plane)[(((int64_t) pt[i] * c.kv + head) * c.page.d + at_t[i]) * per_head + at] = v[i];
-    }
-}
+struct Spot {   // of an entry: its page, and its token of the page
+    int page, in;
+};
 
 template <int TYPE> __global__ void __launch_bounds__(256) kv_move_kernel(Move g, int block0) {
     const int b = block0 + blockIdx.x, cache = b % g.n_caches, grp = b / g.n_caches;
     const KvView& c = g.cache;
     const int e0 = min(max(g.offsets[grp], 0), g.n), e1 = min(max(g.offsets[grp + 1], e0), g.n);
     const int lane = threadIdx.x & 63;
+    const int row = kv_row_bytes(TYPE, c.dim) / 16, codes = c.kv * row, sc = kv_scales(TYPE, c.dim), all = 2 * (codes + c.kv * sc);
     for (int s0 = e0; s0 < e1; s0 += 64) {
         const int e = s0 + lane;
         int f = -1, t = -1;
@@ -288,31 +280,46 @@ template <int TYPE> __global__ void __launch_bounds__(256) kv_move_kernel(Move g
         unsigned long long on = __ballot(f >= 0 && t >= 0 && f < slots && t < slots && f != t);
         while (on) {
             // up to BATCH entries whose sources no earlier one of them writes
-            int pf[BATCH], at_f[BATCH], pt[BATCH], at_t[BATCH], to[BATCH], n = 0;
+            Spot from[BATCH], to[BATCH];
+            int dst[BATCH], n = 0;
 #pragma unroll
             for (int i = 0; i < BATCH; i++) {
-                pf[i] = at_f[i] = pt[i] = at_t[i] = 0, to[i] = -1;
+                from[i] = to[i] = {0, 0}, dst[i] = -1;
                 if (on && n == i) {
                     const int l = __ffsll(on) - 1;
                     const int ff = __builtin_amdgcn_readlane(f, l), tt = __builtin_amdgcn_readlane(t, l);
                     bool clash = false;
 #pragma unroll
-                    for (int j = 0; j < i; j++) clash |= to[j] == ff;
+                    for (int j = 0; j < i; j++) clash |= dst[j] == ff;
                     if (!clash) {
-                        pf[i] = c.page.div(ff), at_f[i] = ff - pf[i] * c.page.d;
-                        pt[i] = c.page.div(tt), at_t[i] = tt - pt[i] * c.page.d;
-                        to[i] = tt;
+                        from[i].page = c.page.div(ff), from[i].in = ff - from[i].page * c.page.d;
+                        to[i].page = c.page.div(tt), to[i].in = tt - to[i].page * c.page.d;
+                        dst[i] = tt;
                         n = i + 1;
                         on &= on - 1;
                     }
                 }
             }
-            const int row = kv_row_bytes(TYPE, c.dim) / 16, sc = kv_scales(TYPE, c.dim);
-            move_pieces<uint4_t>(g.k[cache], 0, c.kv * row, row, c, pf, at_f, pt, at_t, n);
-            move_pieces<uint4_t>(g.v[cache], 0, c.kv * row, row, c, pf, at_f, pt, at_t, n);
-            if (TYPE != F16) {
-                move_pieces<uint16_t>(g.k[cache], c.scale_off, c.kv * sc, sc, c, pf, at_f, pt, at_t, n);
-                move_pieces<uint16_t>(g.v[cache], c.scale_off, c.kv * sc, sc, c, pf, at_f, pt, at_t, n);
+            for (int u = threadIdx.x; u < all; u += blockDim.x) {
+                const bool scale = TYPE != F16 && u >= 2 * codes;
+                const int half = scale ? c.kv * sc : codes, v = scale ? u - 2 * codes : u, p = v >= half ? v - half : v, per = scale ? sc : row;
+                uint8_t* const buf = (v >= half ? g.v[cache] : g.k[cache]) + (scale ? c.scale_off : 0);
+                const int head = p / per, at = p - head * per;
+                auto place = [&](const Spot& s) { return (((int64_t) s.page * c.kv + head) * c.page.d + s.in) * per + at; };
+                uint4_t x[BATCH];
+                uint16_t y[BATCH];
+#pragma unroll
+                for (int i = 0; i < BATCH; i++)
+                    if (i < n) {
+                        if (scale) y[i] = reinterpret_cast<const uint16_t*>(buf)[place(from[i])];
+                        else x[i] = reinterpret_cast<const uint4_t*>(buf)[place(from[i])];
+                    }
+#pragma unroll
+                for (int i = 0; i < BATCH; i++)
+                    if (i < n) {
+                        if (scale) reinterpret_cast<uint16_t*>(buf)[place(to[i])] = y[i];
+                        else reinterpret_cast<uint4_t*>(buf)[place(to[i])] = x[i];
+                    }
             }
         }
     }

@@ -62,40 +62,82 @@ __global__ void __launch_bounds__(64 * WAVES) tree_masks_kernel(Trees g, uint64_
     }
 }
 
-__global__ void __launch_bounds__(64 * WAVES) tree_accept_kernel(Trees g, TreeWalk w) {
+// What a walk reads of a tree: of up to 64 * BLOCKS nodes in the wave's registers, so that a step is a few comparisons and no load; of more
+// (BLOCKS 0) in memory. 256 trees of 64: WALK_US.
+template <int BLOCKS> struct Nodes {
+    int parent[BLOCKS], token[BLOCKS], pick[BLOCKS];
+    JAMHIP_DEV Nodes(const Trees& g, const TreeWalk& w, const Range& r) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++) {
+            const int i = 64 * b + lane;
+            parent[b] = -1, token[b] = pick[b] = 0;
+            if (i < r.nq) parent[b] = g.parents[r.t0 + i], token[b] = w.tokens[r.t0 + i], pick[b] = w.picked[r.t0 + i];
+        }
+    }
+    JAMHIP_DEV int pick_of(int at) const {
+        int v = 0;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; b++)
+            if (at / 64 == b) v = __builtin_amdgcn_readlane(pick[b], at % 64);
+        return v;
+    }
+    // the first child of `at` whose token is v, -1 for none; a child comes after its parent
+    JAMHIP_DEV int child(int at, int v) const {
+        const int lane = threadIdx.x & 63;
+        int found = -1;
+#pragma unroll
+        for (int b = BLOCKS - 1; b >= 0; b--) {
+            const unsigned long long hit = __ballot(parent[b] == at && token[b] == v && 64 * b + lane > at);
+            if (hit) found = 64 * b + __ffsll(hit) - 1;
+        }
+        return found;
+    }
+};
+template <> struct Nodes<0> {
+    const Trees& g;
+    const TreeWalk& w;
+    const Range& r;
+    JAMHIP_DEV Nodes(const Trees& g, const TreeWalk& w, const Range& r) : g(g), w(w), r(r) {}
+    JAMHIP_DEV int pick_of(int at) const { return w.picked[r.t0 + at]; }
+    JAMHIP_DEV int child(int at, int v) const {
+        const int lane = threadIdx.x & 63;
+        for (int b = (at + 1) / 64; 64 * b < r.nq; b++) {
+            const int i = 64 * b + lane;
+            const unsigned long long hit = __ballot(i > at && i < r.nq && g.parents[r.t0 + i] == at && w.tokens[r.t0 + i] == v);
+            if (hit) return 64 * b + __ffsll(hit) - 1;
+        }
+        return -1;
+    }
+};
+
+template <int BLOCKS> __global__ void __launch_bounds__(64 * WAVES) tree_accept_kernel(Trees g, TreeWalk w) {
     const int lane = threadIdx.x & 63, s = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (s >= g.n_seqs) return;
     const Range r = range_of(g, s);
+    const Nodes<BLOCKS> nodes(g, w, r);
     int* path = w.path + (int64_t) s * w.ld_path;
-    int at = 0, n = 0, pick = -1;
-    bool on = r.nq > 0 && w.ld_path > 0;
-    while (on) {
-        pick = w.picked[r.t0 + at];
-        if (lane == 0) {
-            path[n] = at;
-            if (w.from != nullptr) {
-                const bool move = at != n;
-                w.from[r.t0 + n] = move ? w.slots[r.t0 + at] : -1;
-                w.to[r.t0 + n] = move ? w.slots[r.t0 + n] : -1;
+    int at = r.nq > 0 && w.ld_path > 0 ? 0 : -1, n = 0, pick = -1;
+    int mine = -1;   // lane k holds the walk's place k of each 64
+    auto write = [&](int k0, int k1) {   // places [k0, k1) of the path, those past its end as none
+        for (int k = k0 + lane; k < k1; k += 64) {
+            const int c = k < n ? mine : -1;
+            if (k < w.ld_path) path[k] = c;
+            if (w.from != nullptr && k < r.all) {
+                w.from[r.t0 + k] = c > k ? w.slots[r.t0 + c] : -1;   // a place is never below its number; at it nothing moves
+                w.to[r.t0 + k] = c > k ? w.slots[r.t0 + k] : -1;
             }
         }
+    };
+    while (at >= 0) {
+        pick = nodes.pick_of(at);
+        if (lane == n % 64) mine = at;
         n++;
-        on = false;
-        if (n >= w.ld_path) break;
-        for (int b = (at + 1) / 64; 64 * b < r.nq; b++) {   // a child comes after its parent
-            const int i = 64 * b + lane;
-            const bool fits = i > at && i < r.nq && g.parents[r.t0 + i] == at && w.tokens[r.t0 + i] == pick;
-            const unsigned long long hit = __ballot(fits);
-            if (hit) {
-                at = 64 * b + __ffsll(hit) - 1;
-                on = true;
-                break;
-            }
-        }
+        if (n % 64 == 0) write(n - 64, n);
+        at = n < w.ld_path ? nodes.child(at, pick) : -1;
     }
-    for (int k = n + lane; k < w.ld_path; k += 64) path[k] = -1;
-    if (w.from != nullptr)
-        for (int k = n + lane; k < r.all; k += 64) w.from[r.t0 + k] = w.to[r.t0 + k] = -1;
+    const int done = n / 64 * 64, end = max(w.ld_path, r.all);
+    write(done, end);   // past the first 64 of them all are none: n < done + 64
     if (lane == 0) {
         w.accepted[s] = n;
         w.next[s] = pick;
@@ -111,7 +153,10 @@ hipError_t launch_tree_masks(const Trees& g, uint64_t* masks, int words, int* po
 }
 
 hipError_t launch_tree_accept(const Trees& g, const TreeWalk& w, hipStream_t st) {
-    tree_accept_kernel<<<(uint32_t) (((int64_t) g.n_seqs + WAVES - 1) / WAVES), 64 * WAVES, 0, st>>>(g, w);
+    const uint32_t blocks = (uint32_t) (((int64_t) g.n_seqs + WAVES - 1) / WAVES);
+    if (g.max_q <= 64) tree_accept_kernel<1><<<blocks, 64 * WAVES, 0, st>>>(g, w);
+    else if (g.max_q <= 256) tree_accept_kernel<4><<<blocks, 64 * WAVES, 0, st>>>(g, w);
+    else tree_accept_kernel<0><<<blocks, 64 * WAVES, 0, st>>>(g, w);
     return hipGetLastError();
 }
 

@@ -27,10 +27,6 @@ struct TreeSpan {
     int tree0, b0, b1;    // and keys tree0 + j of the bits j in [b0, b1)
 };
 
-struct TreeHull {
-    int lo, hi;   // the first and the last key of a span, lo > hi for none
-};
-
 JAMHIP_MASK_DEV int mask_max(int a, int b) { return a > b ? a : b; }
 JAMHIP_MASK_DEV int mask_min(int a, int b) { return a < b ? a : b; }
 
@@ -81,35 +77,14 @@ JAMHIP_MASK_DEV TreeSpan span_cut(TreeSpan s, int skip, int c0, int c1) {
     return s;
 }
 
-// a range that holds every key of a whole span, [span_lo, span_hi): without a look at the bits
+// a range that holds every key of a span, [span_lo, span_hi), without a look at the bits
 JAMHIP_MASK_DEV int span_lo(const TreeSpan& s) { return s.ctx_lo < s.ctx_hi ? s.ctx_lo : s.tree0 + s.b0; }
-JAMHIP_MASK_DEV int span_hi(const TreeSpan& s) { return s.b0 < s.b1 ? s.tree0 + s.b1 : s.ctx_hi; }
+JAMHIP_MASK_DEV int span_hi(const TreeSpan& s) { return s.b0 < s.b1 ? s.tree0 + s.b1 : s.ctx_lo < s.ctx_hi ? s.ctx_hi : s.tree0 + s.b0; }
 
 JAMHIP_MASK_DEV bool span_sees(const TreeMask& m, const TreeSpan& s, int key) {
     if (key >= s.ctx_lo && key < s.ctx_hi) return true;
     const int j = key - s.tree0;
     return j >= s.b0 && j < s.b1 && (m.row[j / 64] >> (j % 64) & 1);
-}
-
-JAMHIP_MASK_DEV TreeHull span_hull(const TreeMask& m, const TreeSpan& s) {
-    TreeHull h{INT32_MAX, -1};
-    if (s.b0 < s.b1) {
-        for (int w = (s.b1 - 1) / 64; w >= s.b0 / 64; w--)
-            if (const uint64_t v = mask_word(m, w, s.b0, s.b1)) {
-                h.hi = s.tree0 + 64 * w + 63 - __builtin_clzll(v);
-                break;
-            }
-        for (int w = s.b0 / 64; h.hi >= 0 && 64 * w < s.b1; w++)
-            if (const uint64_t v = mask_word(m, w, s.b0, s.b1)) {
-                h.lo = s.tree0 + 64 * w + __builtin_ctzll(v);
-                break;
-            }
-    }
-    if (s.ctx_lo < s.ctx_hi) {
-        h.lo = s.ctx_lo;
-        h.hi = mask_max(h.hi, s.ctx_hi - 1);
-    }
-    return h;
 }
 
 // bit i: the key k0 + i is seen, for the 64 keys from k0 on
