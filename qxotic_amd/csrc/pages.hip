@@ -140,14 +140,13 @@ __global__ void __launch_bounds__(T) kv_resize_kernel(Pages g) {
 // the tokens. A page that one sequence gives back and another takes is looked up where it comes from, so no workgroup waits for another's
 // writes. What may be written in place (lens, held, n_free) is left to a workgroup that nobody reads beside: the only one, or, where the arrays
 // are apart, the first, or a launch of its own behind the others.
-constexpr int SHARE_TOKENS = 2048, SHARE_ENTRIES = 16384;   // of a workgroup: new tokens, entries of the table
+constexpr int SHARE_TOKENS = 1024, SHARE_ENTRIES = 16384;   // of a workgroup: new tokens, entries of the table
 constexpr int MOST_GROUPS = 128;
 
-// the last i in [0, T) with a[i] <= v, a rising from a[0] <= v
-JAMHIP_DEV int find_seq(const int* a, int v) {
+// the last i below 2 * half, a power of two up to T, with a[i] <= v, a rising from a[0] <= v
+JAMHIP_DEV int find_seq(const int* a, int v, int half) {
     int lo = 0;
-#pragma unroll
-    for (int step = T / 2; step > 0; step >>= 1) lo += a[lo + step] <= v ? step : 0;
+    for (int step = half; step > 0; step >>= 1) lo += a[lo + step] <= v ? step : 0;
     return lo;
 }
 
@@ -186,25 +185,26 @@ __global__ void __launch_bounds__(T) kv_resize_shared_kernel(Pages g, bool work,
     s_len[tid] = refused ? -1 - w.len : w.len;
     const int taken = stop < T ? take_at[stop] : total[1];
     __syncthreads();
+    const int half = g.n_seqs > 1 ? 1 << (31 - __builtin_clz(g.n_seqs - 1)) : 0;   // 2 * half >= n_seqs
     // the page at place i of the free list once all are given back
     auto page_at = [&](int i) {
         if (i < free0) return g.free_pages[i];
-        const int k = free0 + total[0] - 1 - i, s = find_seq(back_at, k);
+        const int k = free0 + total[0] - 1 - i, s = find_seq(back_at, k, half);
         return g.seq_pages[(int64_t) s * g.ld + s_need[s] + (k - back_at[s])];
     };
     if (work) {
         for (int k = blockIdx.x * T + tid; k < total[0]; k += gridDim.x * T) {
-            const int s = find_seq(back_at, k), place = free0 + total[0] - 1 - k;
+            const int s = find_seq(back_at, k, half), place = free0 + total[0] - 1 - k;
             if (place < g.free_cap) g.free_pages[place] = g.seq_pages[(int64_t) s * g.ld + s_need[s] + (k - back_at[s])];
         }
         for (int k = blockIdx.x * T + tid; k < taken; k += gridDim.x * T) {
-            const int s = find_seq(take_at, k);
+            const int s = find_seq(take_at, k, half);
             g.seq_pages[(int64_t) s * g.ld + s_held[s] + (k - take_at[s])] = page_at(have - 1 - k);
         }
         for (int t = blockIdx.x * T + tid; t < g.n_tokens; t += gridDim.x * T) {
             int pos = 0, slot = -1;
             if (t < total[2]) {
-                const int s = find_seq(row_at, t), p = (s_len[s] < 0 ? -1 - s_len[s] : s_len[s]) + (t - row_at[s]);
+                const int s = find_seq(row_at, t, half), p = (s_len[s] < 0 ? -1 - s_len[s] : s_len[s]) + (t - row_at[s]);
                 pos = p + (g.base != nullptr ? g.base[s] : 0);
                 if (s_len[s] >= 0) {
                     const int c = g.page.div(p), page = c < s_held[s] ? g.seq_pages[(int64_t) s * g.ld + c] : page_at(have - 1 - (take_at[s] + c - s_held[s]));
