@@ -69,8 +69,9 @@ class Decoder:
     def _norm(x):
         return (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6)).contiguous()
 
-    def forward(self, tokens, positions, slots, batch: AttnBatch):
-        """Logits [n, VOCAB] of the call's tokens: int32 device tensors [n], the batch's arrays on the device too."""
+    def forward(self, tokens, positions, slots, batch: AttnBatch, masks=None):
+        """Logits [n, VOCAB] of the call's tokens: int32 device tensors [n], the batch's arrays on the device too. masks int64 [n, words]: the
+        tokens are drafted trees (examples/tree_step.py)."""
         with torch.cuda.stream(self.stream):
             n, q_dim, kv_dim = tokens.numel(), HEADS * DIM, KV * DIM
             x = self.embedding[tokens.long()].clone()
@@ -80,7 +81,10 @@ class Decoder:
                 k, v = q + 4 * q_dim, q + 4 * (q_dim + kv_dim)
                 self._ok(self.jam.qkv_norm_rope_write(self.spec, cache, q, ld, q, ld, k, ld, v, ld, positions.data_ptr(), slots.data_ptr(), n))
                 seen = torch.zeros((n, q_dim), device="cuda")
-                self._ok(self.jam.attn_shared_prefix(cache, batch, q, ld, HEADS, DIM ** -0.5, seen.data_ptr(), q_dim))
+                if masks is None:
+                    self._ok(self.jam.attn_shared_prefix(cache, batch, q, ld, HEADS, DIM ** -0.5, seen.data_ptr(), q_dim))
+                else:
+                    self._ok(self.jam.attn_tree(cache, batch, masks.data_ptr(), masks.shape[1], q, ld, HEADS, DIM ** -0.5, seen.data_ptr(), q_dim))
                 self._mm(layer["o"], seen, x)
                 up = self._mm(layer["up"], self._norm(x))
                 self._ok(self.jam.glu_device(HipJAM.ACT_SWIGLU, up.data_ptr(), 2 * FFN, up.data_ptr() + 4 * FFN, 2 * FFN, n, FFN))

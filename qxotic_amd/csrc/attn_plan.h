@@ -43,9 +43,10 @@ struct AttnPlan {
 // Splits of up to `longest` keys for `groups` workgroups with work: as many workgroups as are resident at once, two to a CU, whole
 // tiles each. More do not help where sequences differ in length: a run of keys costs its start and end (64 sequences of 33 to
 // 1024 keys, 8 key heads: 27 us as one run each, 31 as two, 36 as four).
-inline int attn_splits(int cfg, int64_t groups, int keys, int longest, int* chunk) {
+// places: the workgroups to make; whole: keys of so many tiles stay in one piece.
+inline int attn_splits(int cfg, int64_t groups, int keys, int longest, int* chunk, int places = 512, int whole = 0) {
     const int tiles = longest > 0 ? up_div(longest, keys) : 1, least = cfg < 2 ? 1 : 2;
-    const int64_t want = groups >= 512 ? 1 : 512 / groups;
+    const int64_t want = groups >= places || tiles <= whole ? 1 : places / groups;
     int splits = (int) (want < tiles / least ? want : tiles / least);
     if (splits < 1) splits = 1;
     const int per = up_div(tiles, splits);
@@ -66,16 +67,22 @@ inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, in
     // behind 3000 45 / 35, 16000 95 / 105; 64 of 32 rows behind 4000 109 / 101, 16000 288 / 357.
     const int64_t saved = (n_seqs - 4 * (int64_t) n_prefixes) * kv * max_prefix, cost = (60000 + 7500 * (int64_t) n_seqs) * (rows <= 8 ? 1 : 4);
     const bool grouped = n_prefixes > 0 && rows < attn_rows(2) && saved >= cost;
+    // Trees, by what there is to do, in pieces of 128 rows and 128 keys of a key head. A few hundred: 32-row tiles, which give more waves something
+    // to do at once, though each reads the keys. Up to 2048: one workgroup a CU, since a second one's parts cost more than it saves, and up to
+    // four tiles of keys in one piece, without a join. In us, 8 key heads, linear batches' rule / this: one tree of 25 over 745 keys (48
+    // pieces, F16, heads of 128) 17.0 / 15.3, 2000 keys (128) 21.0 / 17.9, 8000 (504) 32 / 28; of 63 (Q8_0) 745 keys (96) 20.4 / 16.7, 32000
+    // (4000) 87 / 93 with one a CU, 87 so; eight trees of 32 (F16) 745 keys (384) 28 / 21, 2000 (1024) 38 / 36, 8000 (4032) 92 / 102 with one a CU,
+    // 92 so, 117 in 32-row tiles; four of 25 over 300 keys (96) 17.5 / 13.5, over 745 in one piece 19.8 / 19.1, one of 25 over 745 in one 15.3 / 17.4.
+    const double pieces = (double) ((rows + 127) / 128) * n_seqs * kv * ((max_seq + (int64_t) max_prefix + 127) / 128);   // past 64 bits at the extremes
+    const int cfg = tree && pieces <= 512 && rows > 16 && dim <= ATTN_WIDE_DIM ? 1 : attn_cfg(rows, dim);
+    const int places = tree && pieces <= 2048 ? 256 : 512, whole = places < 512 ? 4 : 0;
     auto add = [&](int mode, int cfg, int64_t tiles, int64_t busy, int longest) {   // busy: tiles with rows
         AttnPart& a = p.part[p.n++];
         a.mode = mode, a.cfg = cfg, a.tiles = (int) tiles, a.slot0 = p.slots;
-        a.splits = attn_splits(cfg, busy * kv, attn_keys(cfg, dim), longest, &a.chunk);
+        a.splits = attn_splits(cfg, busy * kv, attn_keys(cfg, dim), longest, &a.chunk, places, whole);
         p.slots += a.splits;
         fits = fits && tiles <= INT32_MAX / kv / a.splits;
     };
-    // Trees of more rows than that whose 128-row tiles would leave most of the chip idle, however their keys are split
-    const bool few = tree && dim <= ATTN_WIDE_DIM && (rows + 127) / 128 * n_seqs * kv * ((max_seq + (int64_t) max_prefix + 127) / 128) < 256;
-    const int cfg = few && rows > 16 ? 1 : attn_cfg(rows, dim);
     const int64_t per = (rows + attn_rows(cfg) - 1) / attn_rows(cfg);
     if (!grouped) {
         add(0, cfg, per * n_seqs, per * n_seqs, max_seq + max_prefix);

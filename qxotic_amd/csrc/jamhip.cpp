@@ -1517,7 +1517,14 @@ jamhip_ctx* global_ctx() {
 
 // Runs f on ctx, or on the process-global context when ctx is NULL; a failure there records its message for
 // jamhip_last_error(NULL).
-template <class F> jamhip_status on_ctx(jamhip_ctx* ctx, F&& f) {
+template <class F> jamhip_status on_ctx(jamhip_ctx* ctx, F&& call) {
+    auto f = [&](jamhip_ctx* x) {   // no exception (a string or list that finds no memory) passes the C boundary
+        try {
+            return call(x);
+        } catch (...) {
+            return JAMHIP_EINVAL;
+        }
+    };
     if (ctx) return f(ctx);
     jamhip_ctx* g = global_ctx();
     if (!g) return JAMHIP_EINVAL;

@@ -328,13 +328,20 @@ template <int TYPE> __global__ void __launch_bounds__(256) kv_move_kernel(Move g
 }  // namespace
 
 hipError_t launch_kv_resize(const Pages& g, hipStream_t st) {
-    // 64 sequences of 32 new tokens 10.1 us by the kernels for any number, 512 with 113000 tokens and 27000 pages 36.4; SHARED_US here
-    if (g.n_seqs <= T && g.ld < 1 << 20 && g.n_tokens < 1 << 20) {
+    // us a call: 64 sequences of 32 new tokens 5.3, by the kernels for any number 10.1; 512 with 113000 tokens and 27000 pages 8.1, 36.4
+    if (g.n_seqs <= T && g.ld < 1 << 20 && g.n_tokens < 1 << 20 && g.free_cap < 1 << 30) {
         const int64_t want = std::max(((int64_t) g.n_tokens + SHARE_TOKENS - 1) / SHARE_TOKENS,
                                       ((int64_t) g.n_seqs * g.ld + SHARE_ENTRIES - 1) / SHARE_ENTRIES);
         const int groups = (int) std::min<int64_t>(std::max<int64_t>(want, 1), MOST_GROUPS);
-        auto apart = [](const int* a, const int* b, int n) { return a + n <= b || b + n <= a; };
-        const bool one = groups == 1 || (apart(g.lens, g.lens_out, g.n_seqs) && apart(g.held, g.held_out, g.n_seqs) && apart(g.n_free, g.n_free_out, 1));
+        bool one = groups == 1;
+        if (!one) {   // no array that the first workgroup writes is one that others still read
+            auto overlap = [](const int* a, int n, const int* b, int m) { return a < b + m && b < a + n; };
+            const struct { const int* p; int n; } in[] = {{g.lens, g.n_seqs}, {g.targets, g.n_seqs}, {g.held, g.n_seqs}, {g.base, g.base ? g.n_seqs : 0}, {g.n_free, 1}};
+            const struct { const int* p; int n; } out[] = {{g.lens_out, g.n_seqs}, {g.held_out, g.n_seqs}, {g.n_free_out, 1}, {g.status, g.n_seqs}, {g.q_offsets, g.n_seqs + 1}};
+            one = true;
+            for (const auto& i : in)
+                for (const auto& o : out) one = one && !overlap(i.p, i.n, o.p, o.n);
+        }
         kv_resize_shared_kernel<<<groups, T, 0, st>>>(g, true, one);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || one) return e;

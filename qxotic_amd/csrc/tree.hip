@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(64 * WAVES) tree_masks_kernel(Trees g, uint64_
 }
 
 // What a walk reads of a tree: of up to 64 * BLOCKS nodes in the wave's registers, so that a step is a few comparisons and no load; of more
-// (BLOCKS 0) in memory. 256 trees of 64: WALK_US.
+// (BLOCKS 0) in memory. 256 trees of 64: 3.4 us, with a round of loads for every step 6.4.
 template <int BLOCKS> struct Nodes {
     int parent[BLOCKS], token[BLOCKS], pick[BLOCKS];
     JAMHIP_DEV Nodes(const Trees& g, const TreeWalk& w, const Range& r) {

@@ -282,7 +282,8 @@ def test_move_long_offsets(hip):
         if kind == D.F16:
             assert size > 1 << 32
         k = torch.zeros(size, dtype=torch.uint8, device="cuda")
-        c.k = c.v = k.data_ptr()
+        v = torch.zeros(size, dtype=torch.uint8, device="cuda")
+        c.k, c.v = k.data_ptr(), v.data_ptr()
         plane = k[:pages * kv * page * row].view(pages, kv, page, row)
         x = torch.randint(0, 256, (kv, row), dtype=torch.uint8, device="cuda")
         plane[pages - 1, :, 3] = x

@@ -14,7 +14,19 @@ ROOT = Path(__file__).resolve().parent.parent
 SHIM = """
 #include "treemask.h"
 #include "treeargs.h"
+#include "attn_plan.h"
 using namespace jamhip;
+extern "C" void q_plan(int dim, int kv, int grp, int tokens, int seqs, int prefixes, int max_q, int max_seq, int max_prefix, int tree, int* o) {
+    const AttnPlan p = attn_plan(dim, kv, grp, tokens, seqs, prefixes, max_q, max_seq, max_prefix, tree);
+    o[0] = p.n, o[1] = p.slots;
+    for (int i = 0; i < p.n; i++) {
+        const AttnPart& a = p.part[i];
+        int* q = o + 2 + 7 * i;
+        q[0] = a.mode, q[1] = a.cfg, q[2] = a.tiles, q[3] = a.chunk, q[4] = a.splits, q[5] = a.slot0, q[6] = a.direct;
+    }
+}
+extern "C" int q_rows(int cfg) { return attn_rows(cfg); }
+extern "C" int q_keys(int cfg, int dim) { return attn_keys(cfg, dim); }
 // o: the range that holds its keys; sees[n], tiles[n]: 64 bits from key i on
 extern "C" void q_span(const uint64_t* row, int words, int base, int first, int nq, int window, int skip, int c0, int c1, int n, int* o, int* sees, uint64_t* tiles) {
     const TreeMask m{row, words};
@@ -75,6 +87,45 @@ def test_seen_keys(lib):
             assert o[0] <= min(want) and o[1] > max(want)
         if o[0] < o[1]:
             assert c0 <= o[0] and o[1] <= c1
+
+
+def plan(lib, *args):
+    o = (ctypes.c_int * 16)()
+    lib.q_plan(*args, o)
+    keys = ("mode", "cfg", "tiles", "chunk", "splits", "slot0", "direct")
+    return o[1], [dict(zip(keys, o[2 + 7 * i:9 + 7 * i])) for i in range(o[0])]
+
+
+def test_tree_plans(lib):
+    """How calls of drafted trees are cut: every row and key is in one workgroup's run, by whichever rule; and what the rules choose."""
+    r = random.Random(7)
+    seen = set()
+    for _ in range(3000):
+        dim, kv, grp = r.choice([64, 96, 128, 192, 256]), r.choice([1, 2, 8]), r.choice([1, 4, 8, 16])
+        seqs, q = r.choice([1, 4, 64, 200]), r.choice([1, 4, 25, 64, 300])
+        n = r.choice([0, 0, 1, min(4, seqs)])
+        max_seq, prefix = r.choice([1, 128, 129, 745, 4000, 1 << 20]), r.choice([1, 129, 9000]) if n else 0
+        slots, parts = plan(lib, dim, kv, grp, seqs * q, seqs, n, q, max_seq, prefix, 1)
+        assert [p["mode"] for p in parts] in ([0], [1, 2])
+        used = 0
+        for p in parts:
+            rows, keys = lib.q_rows(p["cfg"]), lib.q_keys(p["cfg"], dim)
+            longest = {0: max_seq + prefix, 1: prefix, 2: max_seq}[p["mode"]]
+            assert p["chunk"] % keys == 0 and p["chunk"] * p["splits"] >= longest and (p["splits"] == 1 or p["chunk"] * (p["splits"] - 1) < longest)
+            assert p["tiles"] >= (seqs * q * grp // rows if p["mode"] == 1 else seqs * -(-q * grp // rows)) and (p["cfg"] != 1 or dim <= 192)
+            if p["direct"]:
+                assert len(parts) == 1 and slots == 0 and p["splits"] == 1
+            else:
+                assert p["slot0"] == used
+                used += p["splits"]
+            seen.add((p["mode"], p["cfg"], p["direct"]))
+        assert used == slots
+    assert {(0, c, d) for c in (0, 1, 2) for d in (0, 1)} <= seen and {(m, 2, 0) for m in (1, 2)} & seen
+    cut = lambda *a: [(p["cfg"], p["splits"]) for p in plan(lib, *a)[1]]   # noqa: E731
+    assert cut(128, 8, 4, 25, 1, 0, 25, 745, 0, 1) == [(1, 6)] and cut(128, 8, 4, 25, 1, 0, 25, 745, 0, 0) == [(2, 6)]
+    assert cut(128, 8, 4, 25, 1, 0, 25, 512, 0, 1) == [(1, 1)] and cut(256, 8, 4, 25, 1, 0, 25, 745, 0, 1) == [(2, 12)]
+    assert cut(128, 8, 4, 256, 8, 0, 32, 2000, 0, 1) == [(2, 4)] and cut(128, 8, 4, 256, 8, 0, 32, 8000, 0, 1) == [(2, 8)]
+    assert cut(128, 8, 4, 2048, 64, 0, 32, 4096, 0, 1) == [(2, 1)] and cut(128, 8, 4, 1, 1, 0, 1, 400, 0, 1) == [(0, 1)]
 
 
 def test_binding_sizes(lib):
