@@ -398,3 +398,123 @@ def test_refusals(hip):
     assert hip.tree_accept(Tree(**tree), None, P, TreePath(**path)) == E and hip.tree_accept(Tree(**tree), P, P, TreePath(**{**path, "lens_out": P})) == E
     assert hip.tree_accept(Tree(**{**tree, "n_tokens": 0, "q_offsets": None}), P, P, TreePath(**path)) == E
     assert hip.tree_accept(Tree(**{**tree, "n_seqs": 0}), P, P, TreePath(**path)) == JAM.OK
+
+
+def test_attn_long_offsets(hip):
+    """Pages whose byte offsets pass 32 bits, in a cache of 4.8 GB."""
+    import torch
+    from qxotic_amd.jam import AttnBatch, KvCache
+    kv, dim, page, pages, nq = 8, 128, 64, 36700, 9
+    c = KvCache(type=D.F16, kv_heads=kv, head_dim=dim, page_tokens=page, n_pages=pages)
+    size = hip.kv_cache_bytes(c)
+    assert size > 1 << 32
+    r = np.random.default_rng(0)
+    bufs = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    c.k, c.v = (b.data_ptr() for b in bufs)
+    n, use = 150, [36699, 3, 36650]
+    x = r.standard_normal((2, n, kv, dim)).astype(np.float16)
+    for buf, rows in zip(bufs, x):
+        h = buf.view(torch.float16).view(pages, kv, page, dim)
+        for t in range(n):
+            h[use[t // page], :, t % page] = torch.from_numpy(rows[t]).cuda()
+    q = r.standard_normal((nq, 32 * dim)).astype(np.float32)
+    bits = T.ancestors(draft(r, nq))
+    t = [i32([0, nq]), i32([n]), i32(use), torch.from_numpy(q).cuda(), torch.from_numpy(T.words(bits, 1).view(np.int64)).cuda()]
+    out = torch.zeros((nq, 32 * dim), device="cuda")
+    torch.cuda.synchronize()
+    b = AttnBatch(n_tokens=nq, n_seqs=1, max_q=nq, max_seq_len=n, q_offsets=t[0].data_ptr(), seq_lens=t[1].data_ptr(), seq_pages=t[2].data_ptr(),
+                  ld_seq_pages=3)
+    assert hip.attn_tree(c, b, t[4].data_ptr(), 1, t[3].data_ptr(), 32 * dim, 32, dim ** -0.5, out.data_ptr(), 32 * dim) == 0, hip.last_error()
+    hip.synchronize()
+    got = out.cpu().numpy().reshape(nq, 32, dim)
+    keys = [T.seen(n - nq, nq, s) for s in bits]
+    for h in range(kv):
+        want, mass, big = T.attention(q.reshape(nq, 32, dim)[:, 4 * h:4 * h + 4], x[0][:, h], x[1][:, h], keys, np.float64(np.float32(dim ** -0.5)))
+        assert (np.abs(got[:, 4 * h:4 * h + 4] - want) <= (big * (2.0 ** -18 * mass + 2.0 ** -19))[..., None]).all()
+
+
+def test_a_captured_step(hip):
+    """Pages, masks, acceptance, entries moved and pages given back in one graph: replayed with other trees and picks, and with eager calls of the
+    same context in between, it does what the definitions say."""
+    import torch
+    from qxotic_amd.jam import HipJAM, KvCache, KvPages, Tree, TreePath
+    jam = HipJAM()
+    try:
+        r = np.random.default_rng(8)
+        n, nodes, page, pages, ld, kv, dim = 5, 12, 16, 64, 12, 2, 64
+        rows = n * nodes
+        full = lambda *s: torch.full(s, -9, dtype=torch.int32, device="cuda")   # noqa: E731
+        lens0 = r.integers(1, 90, n)
+        held0 = -(-lens0 // page)
+        order = r.permutation(pages)
+        table0, used = np.full((n, ld), -5, np.int32), 0
+        for i, h in enumerate(held0):
+            table0[i, :h] = order[used:used + h]
+            used += h
+        d = dict(lens=i32(lens0), held=i32(held0), n_free=i32([pages - used]), free=i32(np.concatenate([order[used:], np.full(used, -7)])),
+                 table=i32(table0).view(n, ld), targets=full(n), status=full(n), off=full(n + 1), off2=full(n + 1), pos=full(rows), slots=full(rows),
+                 parents=full(rows), tokens=full(rows), picked=full(rows), path=full(n, nodes), accepted=full(n), next=full(n), before=full(n),
+                 after=full(n), src=full(rows), dst=full(rows), masks=torch.zeros((rows, 1), dtype=torch.int64, device="cuda"))
+        cache = [torch.randint(0, 256, (pages * page * kv * (dim + 4),), dtype=torch.uint8, device="cuda") for _ in range(2)]
+        p = {k: t.data_ptr() for k, t in d.items()}
+        c = KvCache(type=D.Q8_0, kv_heads=kv, head_dim=dim, page_tokens=page, n_pages=pages, k=cache[0].data_ptr(), v=cache[1].data_ptr())
+        common = dict(n_seqs=n, page_tokens=page, n_pages=pages, free_cap=pages, ld_seq_pages=ld, held=p["held"], n_free=p["n_free"], free_pages=p["free"],
+                      seq_pages=p["table"], lens_out=p["lens"], held_out=p["held"], n_free_out=p["n_free"], status=p["status"])
+        up = KvPages(n_tokens=rows, lens=p["before"], targets=p["targets"], q_offsets=p["off"], pos=p["pos"], slots=p["slots"], **common)
+        down = KvPages(n_tokens=0, lens=p["lens"], targets=p["after"], q_offsets=p["off2"], **common)
+        tree = Tree(n_tokens=rows, n_seqs=n, max_q=nodes, q_offsets=p["off"], parents=p["parents"])
+        path = TreePath(ld_path=nodes, path=p["path"], accepted=p["accepted"], next=p["next"], lens=p["before"], lens_out=p["after"], slots=p["slots"],
+                        move_from=p["src"], move_to=p["dst"])
+        stream = torch.cuda.Stream()
+        assert jam.set_stream(stream.cuda_stream) == 0
+
+        def step():
+            with torch.cuda.stream(stream):
+                d["before"].copy_(d["lens"])
+                torch.add(d["lens"], nodes, out=d["targets"])
+                assert jam.kv_resize(up) == 0 and jam.tree_masks(tree, p["masks"], 1, p["pos"]) == 0
+                assert jam.tree_accept(tree, p["tokens"], p["picked"], path) == 0
+                assert jam.kv_move(c, 1, p["off"], n, p["src"], p["dst"], rows) == 0
+                assert jam.kv_resize(down) == 0
+
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        lens, held, table = lens0.tolist(), held0.tolist(), table0.tolist()
+        free = order[used:].tolist()
+        for k in range(5):
+            trees = [draft(r, nodes) for _ in range(n)]
+            tokens, picked = agree(r, trees, vocab=4, share=0.9)
+            for name, v in (("parents", trees), ("tokens", tokens), ("picked", picked)):
+                d[name].copy_(i32([x for t in v for x in t]))
+            before = [b.cpu().numpy() for b in cache]
+            torch.cuda.synchronize()
+            if k % 2:
+                step()
+            else:
+                graph.replay()
+            torch.cuda.synchronize()
+            a, rest = T.resize(page, lens, [v + nodes for v in lens], [0] * n, held, free, table, rows)
+            paths = [T.walk(*x, nodes) for x in zip(trees, tokens, picked)]
+            moves = [[(a["slots"][i * nodes + v], a["slots"][i * nodes + q]) for q, v in enumerate(w) if v != q] for i, (w, _) in enumerate(paths)]
+            b, free = T.resize(page, a["lens"], [v + len(w) for v, (w, _) in zip(lens, paths)], [0] * n, a["held"], rest, a["seq_pages"], 0)
+            lens, held, table = b["lens"], b["held"], b["seq_pages"]
+            got = {x: t.cpu().numpy() for x, t in d.items()}
+            assert got["lens"].tolist() == lens and got["held"].tolist() == held and got["table"].tolist() == table
+            assert got["n_free"][0] == len(free) and got["free"][:len(free)].tolist() == free and got["next"].tolist() == [x for _, x in paths]
+            sets = [s for t in trees for s in T.ancestors(t)]
+            assert np.array_equal(got["masks"].view(np.uint64), T.words(sets, 1))
+            start = [v - len(w) for v, (w, _) in zip(lens, paths)]
+            assert got["pos"].tolist() == [start[i // nodes] + len(s) - 1 for i, s in enumerate(sets)]
+            for buf, was in zip(cache, before):   # codes, then scales
+                now, at = buf.cpu().numpy(), 0
+                for row in (dim, dim // 16):
+                    plane = was[at:at + pages * kv * page * row].reshape(pages, kv, page, row)
+                    for g in moves:
+                        for f, t in g:
+                            plane[t // page, :, t % page] = plane[f // page, :, f % page]
+                    at += plane.size
+                assert np.array_equal(now, was)
+    finally:
+        jam.close()
