@@ -106,7 +106,7 @@ template <int TYPE, int D> __global__ void __launch_bounds__(256) attn_join_kern
 
 // The same for drafted trees. A workgroup joins the heads of one token, whose parts are the same: what is looked up for them once takes longer
 // than the join of a row. 16, 32 or 64 lanes a row, 4 elements each, so that a wave's loads are of 1024 bytes. 464 tokens of 64 heads of 64 in
-// two parts, 15 MB: 24 us with a row a wave, as above.
+// two parts, 15 MB: 9.9 us, 24 with a row a wave, as above.
 template <int D> constexpr int join_lanes() { return D <= 64 ? 16 : D <= 128 ? 32 : 64; }
 template <int D> constexpr int join_heads() { return 4 * (64 / join_lanes<D>()); }   // of a workgroup
 

@@ -4,13 +4,19 @@
 // wave, and walks a run of keys, a tile of keys and values at a time: codes come from the cache into registers while the tile
 // before is computed, are turned into f16 and laid out in shared memory once for all rows.
 //
-// Bound by the matrix cores and the VALU alike, each busy about half of the time: at head_dim 64 a tile costs a wave 1024 cycles of
-// products (two for each, for the halves) and about 1100 of VALU (an exponential of 16 cycles, a fused multiply-add, a sum, a
-// maximum, two conversions and a difference for each of 32 scores a lane), and two waves a SIMD take 3900 for it. 64 sequences of 4 heads
-// behind 8192 tokens in Q8_0, 8 key heads of 128: 31 to 33 us; 8 prompts of up to 256 tokens behind 4096 in F16, heads of 64: 293 to 301 us
-// from card to card (434 to 422 TFLOP/s, counted once) after some fifty calls in a row, 340 to 390 before, while the clock rises. Two halves of
-// shared memory with one barrier a tile took 37.8 for the first, 16 runs of keys for 32 took 38. At head_dim 128 the two halves of
-// the query and the next tile's codes are more than 256 registers: 25 (F16), 14 (Q8_0) and 4 (Q4_0) of them go to scratch, at 256 24 to 33.
+// Bound by the matrix cores, the VALU and the power that both take. Products of 32 x 32 x 16 alone, of ordinary values, run at 1.62 PFLOP/s on this
+// card: the clock falls to 1.6 GHz (of zeros 2.45 PFLOP/s). At head_dim 128 a tile costs a wave 2048 cycles of products (two for each, for the
+// halves), and VALU beside them (turning codes into f16, an exponential, a fused multiply-add, a sum, a maximum, two conversions and a
+// difference for each of 32 scores a lane); two workgroups a CU take 5900 cycles for a tile each at 2.05 GHz (Q4_0), 69 % of them products. 64 sequences of 4
+// heads behind 8192 tokens in Q8_0, 8 key heads of 128: 30 us; 8 prompts of up to 256 tokens behind 4096 in F16, heads of 64: 285 us (446
+// TFLOP/s, counted once) after some fifty calls in a row, more before, while the clock rises; trees of up to 32 tokens of 64 sequences
+// of 200 to 4096 tokens in Q8_0 188, of 63 of four of 20011 to 32771 in Q4_0 229 (458).
+//
+// What made it faster (calls of the trees' 64 sequences and long ones): loads that wait for themselves alone, limits and bounds out of the
+// vector registers, operands a product ahead and a wave's priority in its products, together 236 -> 205 and 276 -> 257. No register goes to
+// scratch. What did not: conversion beside the products, with two halves of shared memory and one barrier a tile, 202 -> 212 and 246 -> 251;
+// equal shares of all keys, cut by the device's lengths and joined, 202 -> 207 (179 and a join of 26) and 257 -> 257; two, three and four
+// times the runs of keys 196 -> 229, 218, 224 and 246 -> 260, 271, 269.
 #pragma once
 
 #include "attn_mma.h"

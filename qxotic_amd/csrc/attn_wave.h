@@ -7,10 +7,10 @@
 // read. The next tile's codes are on their way while one is computed.
 //
 // Bound by memory while all workgroups run, then by the longest sequence: 64 sequences of 33 to 1024 keys in Q8_0, 8 key heads of
-// 128, 28 to 30 us (2.6 TB/s over all, 6 at the start). With 32 rows behind 4 x 24001 tokens in Q4_0, 51 us (2.1 TB/s): the bytes take about 23
+// 128, 26 us (2.9 TB/s over all, 6 at the start). With 32 rows behind 4 x 24001 tokens in Q4_0, 46 us (2.3 TB/s): the bytes take about 23
 // of them, the two products 22, turning codes into f16 (7 instructions for 4) 9, and two waves a SIMD do not overlap the three. One
-// sequence of 745 keys 7.1 us: launch and three rounds of dependent loads (lengths, pages, codes). A workgroup of one tile with a barrier
-// between loads and products took 28.8 and 76.9 for the first two. 32 rows of 128 take all registers: 26 (F16) and 2 (Q4_0) go to scratch.
+// sequence of 745 keys 7.2 us: launch and three rounds of dependent loads (lengths, pages, codes); a tree of 25 tokens of it 12.0. A workgroup of
+// one tile with a barrier between loads and products took 28.8 and 76.9 for the first two. 32 rows of 128 in F16 keep 20 registers in scratch (trees 14).
 #pragma once
 
 #include "attn_mma.h"

@@ -3,7 +3,7 @@
 //   mask(i) = {i} ∪ mask(parent(i)),  depth(i) = |mask(i)| - 1;   path: from node 0 on to the first child whose token is the model's pick
 //
 // A wave holds one tree, 64 nodes at a time in their order: a parent is below its child, so what a node needs of the blocks before is
-// finished when its block begins. Bound by the launch and three rounds of loads.
+// finished when its block begins. Bound by the launch and rounds of dependent loads: masks of one tree 1.6 us, of 256 3.0.
 #include "launch.h"
 
 namespace jamhip {
