@@ -377,7 +377,9 @@ jamhip_status jamhip_attn_shared_prefix(jamhip_ctx* ctx, const jamhip_kv_cache* 
 /* ---- A step with drafted trees: several guesses of the tokens that come next, looked at by the model in one pass. A step is
  * jamhip_kv_resize (room for the drafted tokens, their slots), jamhip_tree_masks, then in every layer jamhip_qkv_norm_rope_write and
  * jamhip_attn_tree, jamhip_sample on every drafted token's logits, jamhip_tree_accept, jamhip_kv_move for all layers at once, and
- * jamhip_kv_resize again, to the accepted lengths. The lengths, tables and counts stay on the device; a captured step can be replayed. */
+ * jamhip_kv_resize again, to the accepted lengths. The lengths, tables and counts stay on the device; a captured step can be replayed. What the
+ * first jamhip_kv_resize refuses goes through the rest without slots: its rows of the pass mean nothing, and jamhip_tree_accept, given the
+ * slots, leaves it as it was, to be tried again in the next step. */
 
 /* Page tables and slots. All arrays are int32 device memory; lens_out, held_out and n_free_out may be lens, held and n_free. */
 typedef struct {
@@ -436,17 +438,19 @@ typedef struct {
     int         ld_path;     /* the longest path */
     void*       path;        /* [n_seqs][ld_path] places of the accepted tokens among their sequence's, rising, then -1 */
     void*       accepted;    /* [n_seqs] their number: at least 1 for a sequence with tokens, if ld_path is */
-    void*       next;        /* [n_seqs] what the model picked at the last of them, -1 for a sequence without tokens */
+    void*       next;        /* [n_seqs] what the model picked at the last of them; the root again for a sequence without slots, -1 for one
+                              * without tokens */
     const void* lens;        /* [n_seqs] lengths before the step; NULL without lens_out */
     void*       lens_out;    /* [n_seqs] lens + accepted, or NULL; may be lens */
-    const void* slots;       /* [n_tokens] the tokens' slots; NULL without move_from */
+    const void* slots;       /* [n_tokens] the tokens' slots, or NULL without move_from: then no sequence may have been refused */
     void*       move_from;   /* [n_tokens] or NULL: for jamhip_kv_move with the same q_offsets, the k-th accepted token's slot */
     void*       move_to;     /* [n_tokens] and the k-th token's; -1 both where nothing moves */
 } jamhip_tree_path;
 
 /* The drafted tokens that the model agrees with: from token 0 of each sequence on, the first child (the lowest) whose token is what was picked
  * at its parent, until there is none. tokens, picked: int32 [n_tokens], the drafted tokens and what the model picks after each. With
- * picks that are samples of the model's own distribution, so are the accepted tokens. */
+ * picks that are samples of the model's own distribution, so are the accepted tokens. A sequence whose token 0 has a slot below zero was refused by
+ * jamhip_kv_resize: nothing was written for it, nothing of it is accepted, and lens_out is lens. */
 jamhip_status jamhip_tree_accept(jamhip_ctx* ctx, const jamhip_tree* tree, const void* tokens_dev, const void* picked_dev,
                                  const jamhip_tree_path* path);
 

@@ -73,6 +73,13 @@ def walk(parents, tokens, picked, longest):
     return path, int(picked[path[-1]])
 
 
+def accept(parents, tokens, picked, slots, longest):
+    """walk, of a sequence whose tokens have these slots: one without a slot for its root was refused, and stays as it was."""
+    if len(parents) and slots[0] < 0:
+        return [], int(tokens[0])
+    return walk(parents, tokens, picked, longest)
+
+
 def seen(ctx, nq, bits, window=0):
     """The keys, in order, that a query token sees whose row has these bits: `ctx` context keys, then nq drafted ones."""
     keys = list(range(ctx)) + [ctx + j for j in sorted(bits) if 0 <= j < nq]

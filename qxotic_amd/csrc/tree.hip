@@ -117,7 +117,9 @@ template <int BLOCKS> __global__ void __launch_bounds__(64 * WAVES) tree_accept_
     const Range r = range_of(g, s);
     const Nodes<BLOCKS> nodes(g, w, r);
     int* path = w.path + (int64_t) s * w.ld_path;
-    int at = r.nq > 0 && w.ld_path > 0 ? 0 : -1, n = 0, pick = -1;
+    // a root without a slot: the sequence was refused its pages, its drafted tokens have no entries and it stays where it was
+    const bool refused = r.nq > 0 && w.slots != nullptr && w.slots[r.t0] < 0;
+    int at = r.nq > 0 && w.ld_path > 0 && !refused ? 0 : -1, n = 0, pick = refused ? w.tokens[r.t0] : -1;
     int mine = -1;   // lane k holds the walk's place k of each 64
     auto write = [&](int k0, int k1) {   // places [k0, k1) of the path, those past its end as none
         for (int k = k0 + lane; k < k1; k += 64) {
