@@ -22,19 +22,29 @@ from qxotic_amd.jam import AttnBatch, HipJAM, KvCache, KvPages, Tree, TreePath  
 
 
 class Trees:
-    """Conversations whose state is on the device: [n] lengths and pages held, [n, width] page tables, the list of free pages."""
+    """Conversations whose state is on the device: [n] lengths and pages held, [n, width] page tables, the list of free pages. All of it is made
+    and used on the decoder's stream, which waits for nothing by itself and nothing for it."""
 
     def __init__(self, decoder: Decoder, pages: int, prompts, width: int = 16):
         self.d, self.n, self.pages, self.width = decoder, len(prompts), pages, width
         i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")   # noqa: E731
-        self.lens, self.held, self.table, self.status = i32(self.n), i32(self.n), i32(self.n, width), i32(self.n)
-        self.free = torch.arange(pages, dtype=torch.int32, device="cuda")
-        self.n_free = torch.full((1,), pages, dtype=torch.int32, device="cuda")
-        self.offsets = i32(self.n + 1)
-        self.caches = (KvCache * LAYERS)(*decoder.caches)
-        self.longest = 0   # of a conversation, as the host knows it: at most
-        logits = self._pass(prompts, None)[0]
-        self.logits = logits[(self.offsets[1:] - 1).long()].contiguous()   # after each prompt's last token
+        with torch.cuda.stream(decoder.stream):
+            self.lens, self.held, self.table, self.status = i32(self.n), i32(self.n), i32(self.n, width), i32(self.n)
+            self.free = torch.arange(pages, dtype=torch.int32, device="cuda")
+            self.n_free = torch.full((1,), pages, dtype=torch.int32, device="cuda")
+            self.offsets = i32(self.n + 1)
+            self.caches = (KvCache * LAYERS)(*decoder.caches)
+            self.longest = 0   # of a conversation, as the host knows it: at most
+            logits = self._pass(prompts, None)[0]
+            logits = logits[(self.offsets[1:] - 1).long()].contiguous()   # after each prompt's last token
+        self.logits = self._out(logits)
+
+    def _out(self, t):
+        """A tensor of the decoder's stream for the caller's, which waits for it; it is not used again while that one still reads it."""
+        caller = torch.cuda.current_stream()
+        caller.wait_stream(self.d.stream)
+        t.record_stream(caller)
+        return t
 
     def _resize(self, targets, rows=0, pos=None, slots=None, old=None):
         """To `targets` [n] tokens each; `old`: where the lengths before stay (else they are followed in place)."""
@@ -76,6 +86,10 @@ class Trees:
         """drafts: each conversation's (tokens, parents), token 0 the one that was picked last. Returns (path, next token) of each, and the
         logits of all drafted tokens. `picked`: the model's picks given from outside, int32 [rows]."""
         tokens, parents = [t for t, _ in drafts], [p for _, p in drafts]
+        self.d.stream.wait_stream(torch.cuda.current_stream())   # u and picked are the caller's
+        for t in (u, picked):
+            if t is not None:
+                t.record_stream(self.d.stream)
         logits, flat, slots, before, tree = self._pass(tokens, parents)
         most = max(len(t) for t in tokens)
         with torch.cuda.stream(self.d.stream):
@@ -96,7 +110,7 @@ class Trees:
         if any(status):
             raise RuntimeError("out of pages")
         self.longest = max(held)
-        return [(p[:k], t) for p, k, t in zip(path, accepted, after)], logits
+        return [(p[:k], t) for p, k, t in zip(path, accepted, after)], self._out(logits)
 
 
 def draft(history, root, width=3, depth=4):
