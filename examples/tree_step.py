@@ -36,6 +36,8 @@ class Trees:
             self.caches = (KvCache * LAYERS)(*decoder.caches)
             self.longest = 0   # of a conversation, as the host knows it: at most
             logits = self._pass(prompts, None)[0]
+            if self.status.any():
+                raise RuntimeError("out of pages")
             logits = logits[(self.offsets[1:] - 1).long()].contiguous()   # after each prompt's last token
         self.logits = self._out(logits)
 
@@ -84,7 +86,8 @@ class Trees:
 
     def step(self, drafts, temperature=0.0, u=None, picked=None):
         """drafts: each conversation's (tokens, parents), token 0 the one that was picked last. Returns (path, next token) of each, and the
-        logits of all drafted tokens. `picked`: the model's picks given from outside, int32 [rows]."""
+        logits of all drafted tokens. A conversation without room for its tree stays as it was: its path is empty, its next token the same one.
+        `picked`: the model's picks given from outside, int32 [rows]."""
         tokens, parents = [t for t, _ in drafts], [p for _, p in drafts]
         self.d.stream.wait_stream(torch.cuda.current_stream())   # u and picked are the caller's
         for t in (u, picked):
@@ -104,11 +107,9 @@ class Trees:
             self.d._ok(self.d.jam.tree_accept(tree, flat.data_ptr(), picked.data_ptr(), p))
             self.d._ok(self.d.jam.kv_move(self.caches, LAYERS, self.offsets.data_ptr(), self.n, src.data_ptr(), dst.data_ptr(), flat.numel()))
             self.offsets = torch.empty_like(self.offsets)   # the next call's own; this one's are still read
-            self._resize(lens)
-            out = [t.cpu() for t in (path, accepted, after, self.lens, self.status)]
-        path, accepted, after, held, status = (t.tolist() for t in out)
-        if any(status):
-            raise RuntimeError("out of pages")
+            self._resize(lens)   # refuses none: no length grows
+            out = [t.cpu() for t in (path, accepted, after, self.lens)]
+        path, accepted, after, held = (t.tolist() for t in out)
         self.longest = max(held)
         return [(p[:k], t) for p, k, t in zip(path, accepted, after)], self._out(logits)
 
