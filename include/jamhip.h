@@ -49,7 +49,7 @@ enum {
 /* status: numerically jam_status (jam.h:81-86; JAM.java:87). */
 typedef enum {
     JAMHIP_OK = 0,
-    JAMHIP_EINVAL = 1,        /* null pointer, m/n/k <= 0, ldw < k, lda < k, ldc < m, HIP failure */
+    JAMHIP_EINVAL = 1,        /* null pointer, m/n/k <= 0, ldw < k, lda < k, ldc < m, HIP failure, no host memory */
     JAMHIP_EUNSUPPORTED = 2,  /* dtype combination or block misalignment; caller falls back */
     JAMHIP_EBUSY = 3          /* another call is in flight on this context */
 } jamhip_status;

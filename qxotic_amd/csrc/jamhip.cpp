@@ -16,6 +16,7 @@
 #include "common.h"
 #include "gguf.h"
 #include "launch.h"
+#include "noexcept_call.h"
 #include "treeargs.h"
 
 using namespace jamhip;
@@ -1515,21 +1516,24 @@ jamhip_ctx* global_ctx() {
     return g_global;
 }
 
-// Runs f on ctx, or on the process-global context when ctx is NULL; a failure there records its message for
-// jamhip_last_error(NULL).
+// Runs call on ctx, or on the process-global context when ctx is NULL; a failure there records its message for
+// jamhip_last_error(NULL). An exception (a string or list that finds no memory) is a failure with a message too.
 template <class F> jamhip_status on_ctx(jamhip_ctx* ctx, F&& call) {
-    auto f = [&](jamhip_ctx* x) {   // no exception (a string or list that finds no memory) passes the C boundary
-        try {
-            return call(x);
-        } catch (...) {
-            return JAMHIP_EINVAL;
-        }
+    auto on = [&](jamhip_ctx* x) {
+        return noexcept_call([&] { return call(x); }, [&](const char* text) {
+            std::lock_guard<std::mutex> lk(x->err_mu);
+            x->err = text;
+        });
     };
-    if (ctx) return f(ctx);
-    jamhip_ctx* g = global_ctx();
+    if (ctx) return on(ctx);
+    jamhip_ctx* g = nullptr;
+    (void) noexcept_call([&] { return (g = global_ctx()) ? JAMHIP_OK : JAMHIP_EINVAL; }, [](const char* text) { set_null_error(text); });
     if (!g) return JAMHIP_EINVAL;
-    const jamhip_status st = f(g);
-    if (st != JAMHIP_OK) set_null_error(error_of(g));
+    const jamhip_status st = on(g);
+    if (st != JAMHIP_OK) {
+        std::lock_guard<std::mutex> lk(g->err_mu);
+        set_null_error(g->err);
+    }
     return st;
 }
 
