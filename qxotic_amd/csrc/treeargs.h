@@ -51,6 +51,7 @@ inline Refusal refuse_path(const jamhip_tree* t, const void* tokens, const void*
     if ((p->lens_out != nullptr) && !p->lens) return {JAMHIP_EINVAL, "tree_accept: lens_out without lens"};
     if ((p->move_from != nullptr) != (p->move_to != nullptr) || (p->move_from && !p->slots))
         return {JAMHIP_EINVAL, "tree_accept: move_from and move_to go together, with slots"};
+    if (p->ld_path > MAX_TOKENS) return {JAMHIP_EUNSUPPORTED, "tree_accept: paths beyond 32 bits"};
     return TAKEN;
 }
 
