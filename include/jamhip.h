@@ -456,8 +456,8 @@ jamhip_status jamhip_tree_accept(jamhip_ctx* ctx, const jamhip_tree* tree, const
 
 /* Entry i, keys and values, goes from slot from[i] to slot to[i] (int32 [n]) in each of n_caches caches of one shape. Group j is the entries
  * [offsets[j], offsets[j + 1]); those of a group are moved in their order, groups and caches at once: a slot that one group writes belongs
- * to no other, and every keys and values buffer is there once. An entry with a slot outside the cache is left out. n_groups at most 2^20 and n_groups * n_caches below 2^31 (else
- * JAMHIP_EUNSUPPORTED). */
+ * to no other, and every keys and values buffer is there once. An entry with a slot outside the cache is left out. n_groups at most 2^20 (else
+ * JAMHIP_EUNSUPPORTED), caches any number. */
 jamhip_status jamhip_kv_move(jamhip_ctx* ctx, const jamhip_kv_cache* caches, int n_caches, const void* offsets_dev, int n_groups,
                              const void* from_dev, const void* to_dev, int n);
 

@@ -358,9 +358,8 @@ hipError_t launch_kv_resize(const Pages& g, hipStream_t st) {
 }
 
 hipError_t launch_kv_move(int type, const Move& g, hipStream_t st) {
-    const int64_t blocks = (int64_t) g.groups * g.n_caches;
+    const int64_t blocks = (int64_t) g.groups * g.n_caches;   // at most 2^20 * MOVE_CACHES
     constexpr int64_t RUN = 1 << 23;   // HIP takes fewer than 2^32 threads a launch
-    if (blocks > INT32_MAX) return hipErrorNotSupported;
     for (int64_t b = 0; b < blocks; b += RUN) {
         const uint32_t n = (uint32_t) (blocks - b < RUN ? blocks - b : RUN);
         switch (type) {

@@ -35,3 +35,12 @@ def test_longest_path(lib):
 
     most = (1 << 31) - 1 - 4096
     assert call(1) == call(most) == OK and call(most + 1) == call((1 << 31) - 64) == call((1 << 31) - 1) == U
+
+
+def test_many_groups_of_many_caches(lib):
+    """Any number of caches goes with the largest number of groups: they are launched some at a time."""
+    from qxotic_amd.jam import KvCache
+    shape = dict(type=8, kv_heads=2, head_dim=64, page_tokens=16, n_pages=4, k=P, v=P)
+    caches = (KvCache * 2049)(*(KvCache(**shape) for _ in range(2049)))
+    a = ctypes.c_void_p(P)
+    assert lib.q_move(caches, 2049, a, 1 << 20, a, a, 1) == OK and lib.q_move(caches, 2049, a, (1 << 20) + 1, a, a, 1) == U
