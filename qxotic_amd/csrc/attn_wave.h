@@ -212,7 +212,8 @@ template <int TYPE, int D, int NC, bool TREE> __global__ void __launch_bounds__(
             weight_halves<NC>(sc, u, ph, pl);
             add_values<NC, T::DT, T::STRIDE, M>(o, lv, u, ph, pl);
         }
-        if (lane < T::KEYS) rw[buf ^ 1][lane] = key_at<TYPE, D>(g.cache, after, kvh);
+        // only where the walk gets there: 512 sequences of up to 500 keys, heads of 64 in Q4_0, 33.8 us, with it for every tile 34.3
+        if (lane < T::KEYS && k0 + 2 * step < hi) rw[buf ^ 1][lane] = key_at<TYPE, D>(g.cache, after, kvh);
         sync();   // and read, before the next tile's take their place
     }
 
