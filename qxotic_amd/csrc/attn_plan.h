@@ -40,9 +40,11 @@ struct AttnPlan {
     int slots;      // workspace results per output row
 };
 
-// Splits of up to `longest` keys for `groups` workgroups with work: as many workgroups as are resident at once, two to a CU, whole
-// tiles each. More do not help where sequences differ in length: a run of keys costs its start and end (64 sequences of 33 to
-// 1024 keys, 8 key heads: 27 us as one run each, 31 as two, 36 as four).
+// Splits of up to `longest` keys for `groups` workgroups with work: two workgroups a CU, whole tiles each. More do not help where sequences differ in length: a run of keys costs its start and end (64 sequences of 33 to
+// 1024 keys, 8 key heads: 27 us as one run each, 31 as two, 36 as four). Two for every head size, though by their registers three 128-row tiles of
+// heads of 64 fit a CU and one of heads of 192 and 256; us at 256 / 512 / 768 / 1024 workgroups, trees of four heads a key head: four of 63 tokens over
+// 30000 keys, heads of 64 (Q8_0) 179 / 147 / 146 / 151, 96 (F16) 253 / 193 / 223 / 206, 128 (Q4_0) 275 / 237 / 252 / 247, 192 (Q4_0) 519 / 538 / 556 /
+// 569, 256 (Q8_0) 591 / 608 / 630 / 648; eight of 32 over 8000, 256 (Q8_0) 183 / 203 / 221 / 238: the largest heads would do better with 256.
 // places: the workgroups to make; whole: keys of so many tiles stay in one piece.
 inline int attn_splits(int cfg, int64_t groups, int keys, int longest, int* chunk, int places = 512, int whole = 0) {
     const int tiles = longest > 0 ? up_div(longest, keys) : 1, least = cfg < 2 ? 1 : 2;
@@ -64,7 +66,11 @@ inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, in
     // own rows fill a 16-row tile, since their products stay. In us, grouped against sequence by sequence, Q8_0, heads of 128, 8 key
     // heads and 4 rows unless said: 64 sequences behind 400 tokens 32 / 20, 800 32 / 27, 2000 34 / 49; 16 behind 800 22 / 16, 2000
     // 24 / 24; 4 behind 6000 25 / 19; 64 behind 2000 with 2 key heads 28 / 24, with 1 27 / 19, of 16 rows 60 / 50; 16 of 32 rows
-    // behind 3000 45 / 35, 16000 95 / 105; 64 of 32 rows behind 4000 109 / 101, 16000 288 / 357.
+    // behind 3000 45 / 35, 16000 95 / 105; 64 of 32 rows behind 4000 109 / 101, 16000 288 / 357. Trees go by the same rule; Q8_0, heads of 128, own lengths
+    // up to 600: of 25 tokens (100 rows) 16 sequences behind 4000 99 / 86, 8000 150 / 144, 16000 250 / 256, 64 behind 4000 286 / 264, 8000 480 / 490;
+    // of 8 (32 rows) 16 behind 8000 69 / 61, 16000 98 / 102, 64 behind 4000 112 / 103, 8000 170 / 185; of 4 (16 rows) 64 behind 4000 74 / 78, 8000 104 /
+    // 140. It takes the group too early for heads of 64 (F16, 96 rows, 64 behind 8000 277 / 251) and for few sequences of up to 8 rows (F16,
+    // heads of 128, 8 behind 4000 35 / 23, 8000 37 / 32, 16000 43 / 49).
     const int64_t saved = (n_seqs - 4 * (int64_t) n_prefixes) * kv * max_prefix, cost = (60000 + 7500 * (int64_t) n_seqs) * (rows <= 8 ? 1 : 4);
     const bool grouped = n_prefixes > 0 && rows < attn_rows(2) && saved >= cost;
     // Trees, by what there is to do, in pieces of 128 rows and 128 keys of a key head. A few hundred: 32-row tiles, which give more waves something
@@ -72,7 +78,9 @@ inline AttnPlan attn_plan(int dim, int kv, int grp, int n_tokens, int n_seqs, in
     // four tiles of keys in one piece, without a join. In us, 8 key heads, linear batches' rule / this: one tree of 25 over 745 keys (48
     // pieces, F16, heads of 128) 17.0 / 15.3, 2000 keys (128) 21.0 / 17.9, 8000 (504) 32 / 28; of 63 (Q8_0) 745 keys (96) 20.4 / 16.7, 32000
     // (4000) 87 / 93 with one a CU, 87 so; eight trees of 32 (F16) 745 keys (384) 28 / 21, 2000 (1024) 38 / 36, 8000 (4032) 92 / 102 with one a CU,
-    // 92 so, 117 in 32-row tiles; four of 25 over 300 keys (96) 17.5 / 13.5, over 745 in one piece 19.8 / 19.1, one of 25 over 745 in one 15.3 / 17.4.
+    // 92 so, 117 in 32-row tiles; four of 25 over 300 keys (96) 17.5 / 13.5, over 745 in one piece 19.8 / 19.1, one of 25 over 745 in one 15.3 / 17.4. A
+    // grouped call has so few pieces only with 8 to 19 sequences of up to 8 rows, and is then the same either way (10 behind 2900, F16 29.4 / 29.5;
+    // four heads a key head, Q4_0 33.7 / 32.5).
     const double pieces = (double) ((rows + 127) / 128) * n_seqs * kv * ((max_seq + (int64_t) max_prefix + 127) / 128);   // past 64 bits at the extremes
     const int cfg = tree && pieces <= 512 && rows > 16 && dim <= ATTN_WIDE_DIM ? 1 : attn_cfg(rows, dim);
     const int places = tree && pieces <= 2048 ? 256 : 512, whole = places < 512 ? 4 : 0;

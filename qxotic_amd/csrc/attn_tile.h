@@ -7,10 +7,13 @@
 // Bound by the matrix cores, the VALU and the power that both take. Products of 32 x 32 x 16 alone, of ordinary values, run at 1.62 PFLOP/s on this
 // card: the clock falls to 1.6 GHz (of zeros 2.45 PFLOP/s). At head_dim 128 a tile costs a wave 2048 cycles of products (two for each, for the
 // halves), and VALU beside them (turning codes into f16, an exponential, a fused multiply-add, a sum, a maximum, two conversions and a
-// difference for each of 32 scores a lane); two workgroups a CU take 5900 cycles for a tile each at 2.05 GHz (Q4_0), 69 % of them products. 64 sequences of 4
+// difference for each of 32 scores a lane). Two workgroups of a CU get through a tile every 3350 cycles between them (Q4_0, at 2.1 GHz; 61 % products where
+// all 128 rows are there), one alone takes 5100. Over whole launches of trees the products take 30 to 40 % of the cycles, 41 to 48 % of those in which a
+// CU has work: 5 to 8 us pass before the first tile, waves whose rows a tree does not fill rest, CUs have unequal numbers of tiles, and of two
+// workgroups on a CU one ends first and leaves the other alone. 64 sequences of 4
 // heads behind 8192 tokens in Q8_0, 8 key heads of 128: 30 us; 8 prompts of up to 256 tokens behind 4096 in F16, heads of 64: 285 us (446
 // TFLOP/s, counted once) after some fifty calls in a row, more before, while the clock rises; trees of up to 32 tokens of 64 sequences
-// of 200 to 4096 tokens in Q8_0 188, of 63 of four of 20011 to 32771 in Q4_0 229 (458).
+// of 200 to 4096 tokens in Q8_0 188 to 195, of 63 of four of 20011 to 32771 in Q4_0 229 to 237 (458 to 443).
 //
 // What made it faster (calls of the trees' 64 sequences and long ones): loads that wait for themselves alone, limits and bounds out of the
 // vector registers, operands a product ahead and a wave's priority in its products, together 236 -> 205 and 276 -> 257. No register goes to

@@ -261,7 +261,8 @@ __global__ void __launch_bounds__(FILL) kv_slots_kernel(Pages g) {
 // order without a barrier between them. Pieces are 16 bytes of codes, and scales one by one (their rows are 2, 4, 6 bytes and so on): keys'
 // codes, values' codes, keys' scales, values' scales, numbered through, so that all of an entry is loaded before the first is stored. 64
 // sequences' 6 entries in 32 F16 caches, 101 MB read and written: 18.5 us (5.4 TB/s); one sequence's in 4 Q8_0 caches 4.3 us, rounds of dependent
-// loads (offsets, slots, entries), 6.3 with a plane of the cache after the other.
+// loads (offsets, slots, entries), 6.3 with a plane of the cache after the other. Scales cost more than their bytes, two of them a thread: calls one
+// after another take 21.7 us for the 64 in F16 (101 MB), 20.6 in Q8_0 (54 MB), 15.8 in Q4_0 (28 MB).
 constexpr int BATCH = 4;
 
 struct Spot {   // of an entry: its page, and its token of the page
@@ -330,7 +331,7 @@ template <int TYPE> __global__ void __launch_bounds__(256) kv_move_kernel(Move g
 }  // namespace
 
 hipError_t launch_kv_resize(const Pages& g, hipStream_t st) {
-    // us a call: 64 sequences of 32 new tokens 5.3, by the kernels for any number 10.1; 512 with 113000 tokens and 27000 pages 8.1, 36.4
+    // us a call: 64 sequences of 32 new tokens 5.3, by the kernels for any number 10.1; 512 with 114594 new tokens and 26000 to 30000 pages moved 8.1, 36.4
     if (g.n_seqs <= T && g.ld < 1 << 20 && g.n_tokens < 1 << 20 && g.free_cap < 1 << 30) {
         const int64_t want = std::max(((int64_t) g.n_tokens + SHARE_TOKENS - 1) / SHARE_TOKENS,
                                       ((int64_t) g.n_seqs * g.ld + SHARE_ENTRIES - 1) / SHARE_ENTRIES);
