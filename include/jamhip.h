@@ -437,7 +437,7 @@ jamhip_status jamhip_attn_tree(jamhip_ctx* ctx, const jamhip_kv_cache* cache, co
 typedef struct {
     int         ld_path;     /* the longest path; above 2^31 - 4097 JAMHIP_EUNSUPPORTED */
     void*       path;        /* [n_seqs][ld_path] places of the accepted tokens among their sequence's, rising, then -1 */
-    void*       accepted;    /* [n_seqs] their number: at least 1 for a sequence with tokens, if ld_path is */
+    void*       accepted;    /* [n_seqs] their number: at least 1 for a sequence with tokens and slots, if ld_path is */
     void*       next;        /* [n_seqs] what the model picked at the last of them; the root again for a sequence without slots, -1 for one
                               * without tokens */
     const void* lens;        /* [n_seqs] lengths before the step; NULL without lens_out */
